@@ -190,8 +190,8 @@ def _prepare_attention(case, gen):
         "group_start": _ints(group_start),
         "shared_lens": _ints(shared),
         "scale": dim**-0.5,
-        "max_context": max(context),
         "max_shared": max(shared),
+        "max_own": max(behind),
         "max_query": max(brings),
     }
 
@@ -250,7 +250,7 @@ def run(state):
             return ops.attention_shared_prefix(
                 state["q"], state["key_pool"], state["value_pool"], block_table=state["block_table"], query_start=state["query_start"],
                 context_lens=state["context_lens"], group_start=state["group_start"], shared_lens=state["shared_lens"],
-                scale=state["scale"], max_context=state["max_context"], max_shared=state["max_shared"], max_query=state["max_query"])
+                scale=state["scale"], max_shared=state["max_shared"], max_own=state["max_own"], max_query=state["max_query"])
         if op == "copy":
             ops.copy_pages([state["keys"], state["values"]], state["source"], state["destination"])
             return state["keys"], state["values"]
