@@ -12,6 +12,7 @@ import dataclasses
 import json
 import os
 import warnings
+from collections.abc import Sequence
 from pathlib import Path
 
 import torch
@@ -25,6 +26,9 @@ __all__ = [
     "QueryTiles",
     "attention",
     "attention_calls",
+    "attention_shared_prefix",
+    "can_share_prefix",
+    "copy_pages",
     "forced_product",
     "hipblaslt_build",
     "library_product_bucket",
@@ -53,6 +57,7 @@ __all__ = [
     "sample_rows",
     "silu_mul",
     "time_library_product",
+    "verify_drafts",
 ]
 
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}
@@ -76,6 +81,16 @@ def _check(tensor: torch.Tensor, name: str, *, dtype: torch.dtype | None = None,
         raise KernelError(f"{name} must be {dtype}, not {tensor.dtype}.")
     if shape is not None and tuple(tensor.shape) != tuple(shape):
         raise KernelError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}.")
+
+
+def _check_on_current_device(**tensors: torch.Tensor | None) -> None:
+    """All on the GPU that is current: kernels are launched there, on its current stream."""
+
+    current = torch.cuda.current_device()
+    for name, tensor in tensors.items():
+        if tensor is not None and tensor.device.index != current:
+            raise KernelError(f"{name} lives on {tensor.device}, the current device is cuda:{current}; "
+                              "make the tensors' device current (torch.cuda.device).")
 
 
 def _ptr(tensor: torch.Tensor | None) -> int | None:
@@ -277,7 +292,7 @@ def query_tiles_host(query_lens, query_start, decode_prefix: int, first_position
 # calls of attention() served by each kernel since the import; a bfloat16 call that no
 # matrix-core kernel takes is served by the generic one, many times slower, and is
 # reported once per geometry
-attention_calls = {"decode": 0, "prefill": 0, "generic": 0}
+attention_calls = {"decode": 0, "prefill": 0, "generic": 0, "shared": 0}
 _reported_fallbacks: set = set()
 
 
@@ -408,6 +423,155 @@ def attention(
          _ptr(positions), _ptr(out), n, heads, kv_heads, head_dim, block_size, max_blocks, float(scale),
          window, _code(q.dtype), _stream())
     return out
+
+
+def can_share_prefix(head_dim: int, block_size: int) -> bool:
+    """Whether :func:`attention_shared_prefix` takes this geometry."""
+
+    return bool(load().ms_attention_shared_prefix_supported(head_dim, block_size))
+
+
+def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, per_token: int, max_shared: int,
+                         max_own: int, max_query: int) -> tuple[int, int, int, int]:
+    """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
+    the parts those keys are cut into, the workgroups that share a sequence's tiles of 16
+    rows, and the parts that its own keys are cut into.  ``rows``: tokens times query heads
+    of a kv head."""
+
+    target = _decode_target()
+    tile = 16 if rows <= 16 * groups else 32
+    tiles = max(groups, -(-rows // tile))
+    shared_splits = max(1, min(-(-target // (tiles * kv_heads)), -(-max_shared // 128), _DECODE_MAX_SPLITS))
+    own_tiles = -(-max_query * per_token // 16)
+    own_splits = max(1, min(-(-target // (sequences * own_tiles * kv_heads)), max_own // 160, _DECODE_MAX_SPLITS))
+    return tile, shared_splits, own_tiles, own_splits
+
+
+def attention_shared_prefix(
+    q: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    *,
+    block_table: torch.Tensor,
+    query_start: torch.Tensor,
+    context_lens: torch.Tensor,
+    group_start: torch.Tensor,
+    shared_lens: torch.Tensor,
+    scale: float,
+    max_shared: int | None = None,
+    max_own: int | None = None,
+    max_query: int | None = None,
+) -> torch.Tensor:
+    """Causal attention as :func:`attention` for sequences that share the front of their
+    cache, whose keys and values are read once a group instead of once a sequence.
+
+    ``q [N, heads, head_dim]``, pools and ``block_table [S, max_blocks]`` (int32) as there.
+    Sequence ``s`` brings the tokens ``query_start[s] .. query_start[s + 1] - 1``, the last
+    ``query_start[s + 1] - query_start[s]`` of its ``context_lens[s]`` positions, each of
+    which sees the keys up to its own.  Group ``g`` is the sequences ``group_start[g] ..
+    group_start[g + 1] - 1``, whose first ``shared_lens[g]`` keys are the same and lie
+    before every token that they bring; they are read through the table of the group's
+    first sequence.  A sequence in no group shares nothing; groups and sequences may be
+    empty.  All four are int32 on the device, so that a recorded graph serves other
+    lengths and groups of the same sizes on every replay.
+
+    ``max_shared``, ``max_own`` (keys behind the shared ones) and ``max_query`` (tokens a
+    sequence brings) say how long things are at most, for the cut of the work; results do
+    not hang on them beyond rounding.  A token that sees no key gives zeros, as do rows of
+    ``q`` behind the last sequence.  The caller guarantees that every page that the tables
+    name for the keys that are read lies inside the pool.
+
+    Takes float32 and bfloat16, head sizes in steps of 16 up to 128 and pages of a multiple
+    of 16 keys (:func:`can_share_prefix`), and no window: a window hides most of a long
+    prefix, and :func:`attention` does not read what it hides."""
+
+    _check(q, "q")
+    if q.ndim != 3 or q.numel() == 0:
+        raise KernelError("attention_shared_prefix: q must be [N>0, heads>0, head_dim>0].")
+    n, heads, head_dim = q.shape
+    _check(key_pool, "key_pool", dtype=q.dtype)
+    if key_pool.ndim != 4 or key_pool.shape[3] != head_dim or key_pool.numel() == 0:
+        raise KernelError(
+            f"attention_shared_prefix: pool {tuple(key_pool.shape)} is not [pages, kv_heads, block_size, {head_dim}]."
+        )
+    _check(value_pool, "value_pool", dtype=q.dtype, shape=_value_pool_shape(key_pool))
+    _, kv_heads, block_size, _ = key_pool.shape
+    if heads % kv_heads != 0:
+        raise KernelError(f"attention_shared_prefix: {heads} query heads are not a multiple of {kv_heads} kv heads.")
+    _check(block_table, "block_table", dtype=torch.int32)
+    if block_table.ndim != 2 or block_table.numel() == 0:
+        raise KernelError("attention_shared_prefix: block_table must be [S>0, max_blocks>0].")
+    sequences, max_blocks = block_table.shape
+    _check(query_start, "query_start", dtype=torch.int32, shape=(sequences + 1,))
+    _check(context_lens, "context_lens", dtype=torch.int32, shape=(sequences,))
+    _check(group_start, "group_start", dtype=torch.int32)
+    if group_start.ndim != 1 or group_start.numel() < 2:
+        raise KernelError("attention_shared_prefix: group_start must be [groups + 1] for at least one group.")
+    groups = group_start.numel() - 1
+    _check(shared_lens, "shared_lens", dtype=torch.int32, shape=(groups,))
+    _check_on_current_device(q=q, key_pool=key_pool, value_pool=value_pool, block_table=block_table, query_start=query_start,
+                             context_lens=context_lens, group_start=group_start, shared_lens=shared_lens)
+    longest = max_blocks * block_size
+    bounds = []
+    for name, given, most in (("max_shared", max_shared, longest), ("max_own", max_own, longest), ("max_query", max_query, n)):
+        if given is not None and (type(given) is not int or given < 0):
+            raise KernelError(f"attention_shared_prefix: {name} must be a whole number or None, not {given!r}.")
+        bounds.append(max(1, most if given is None else min(given, most)))
+    per_token = heads // kv_heads
+    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, groups, sequences, kv_heads, per_token, *bounds)
+    out = torch.empty_like(q)
+    slots = shared_splits + own_splits
+    partial_o = torch.empty((n, heads, slots, head_dim), dtype=torch.float32, device=q.device)
+    partial_ml = torch.empty((n, heads, slots, 2), dtype=torch.float32, device=q.device)
+    call("ms_attention_shared_prefix", _ptr(q), _ptr(key_pool), _ptr(value_pool), _ptr(block_table), _ptr(query_start),
+         _ptr(context_lens), _ptr(group_start), _ptr(shared_lens), _ptr(out), _ptr(partial_o), _ptr(partial_ml), n, sequences,
+         groups, heads, kv_heads, head_dim, block_size, max_blocks, float(scale), tile, shared_splits, own_tiles, own_splits,
+         _code(q.dtype), _stream())
+    attention_calls["shared"] += 1
+    return out
+
+
+def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination: Sequence[int]) -> None:
+    """``pool[:, destination[i]] = pool[:, source[i]]`` for every pool ``[calls, pages, ...]``
+    of ``pools`` and every ``i``, in one launch for up to 480 pages.
+
+    The page numbers are the cache manager's, on the host; they travel with the launch, so
+    nothing is copied to the device first (a recorded graph keeps the numbers it was
+    recorded with).  A page may be copied to several others; a destination is named once and
+    is no source."""
+
+    if not isinstance(pools, (list, tuple)) or not pools:
+        raise KernelError("copy_pages takes a list of at least one pool.")
+    for index, pool in enumerate(pools):
+        _check(pool, f"pools[{index}]")
+        if pool.ndim < 3 or pool.numel() == 0:
+            raise KernelError(f"copy_pages: pools[{index}] {tuple(pool.shape)} is not [calls>0, pages>0, ...].")
+    _check_on_current_device(**{f"pools[{index}]": pool for index, pool in enumerate(pools)})
+    count = len(source)
+    if len(destination) != count:
+        raise KernelError(f"copy_pages: {count} pages to {len(destination)} places.")
+    if count == 0:
+        return
+    for page in (*source, *destination):
+        if type(page) is not int:
+            raise KernelError(f"copy_pages: a page is named by a whole number, not {page!r}.")
+    fewest = min(pool.shape[1] for pool in pools)
+    if min(source) < 0 or max(source) >= fewest or min(destination) < 0 or max(destination) >= fewest:
+        raise KernelError(f"copy_pages: a page lies outside the pools' {fewest}.")
+    places = set(destination)
+    if len(places) != count:
+        raise KernelError("copy_pages: a page is the destination of two copies.")
+    if not places.isdisjoint(source):
+        raise KernelError("copy_pages: a page is the source of one copy and the destination of another.")
+    from_pages, to_pages = (ctypes.c_int32 * count)(*source), (ctypes.c_int32 * count)(*destination)
+    most = int(load().ms_copy_pages_most_pools())
+    for first in range(0, len(pools), most):
+        some = pools[first : first + most]
+        bases = (ctypes.c_void_p * len(some))(*(pool.data_ptr() for pool in some))
+        page_bytes = (ctypes.c_int64 * len(some))(*(pool[0, 0].numel() * pool.element_size() for pool in some))
+        calls = (ctypes.c_int32 * len(some))(*(pool.shape[0] for pool in some))
+        pages = (ctypes.c_int32 * len(some))(*(pool.shape[1] for pool in some))
+        call("ms_copy_pages", bases, page_bytes, calls, pages, len(some), from_pages, to_pages, count, _stream())
 
 
 _EPILOGUE_BF16, _EPILOGUE_F32, _EPILOGUE_ADD_F32, _EPILOGUE_SILU_MUL = 0, 1, 2, 3
@@ -886,3 +1050,62 @@ def sample_rows(
     call("ms_sample_rows", _ptr(logits), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(uniform), _ptr(out),
          rows, vocab, _stream())
     return out
+
+
+def verify_drafts(
+    logits: torch.Tensor,
+    row_start: torch.Tensor,
+    draft_tokens: torch.Tensor,
+    *,
+    draft_probs: torch.Tensor | None = None,
+    accept_uniform: torch.Tensor | None = None,
+    draw_uniform: torch.Tensor | None = None,
+    temperature: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target takes, and the token that it gives behind them.
+
+    Request ``r`` has the rows ``row_start[r] .. row_start[r + 1] - 1`` (int32 ``[requests +
+    1]``, from 0 to R) of the target's float32 ``logits [R, V]``: one for each of its drafted
+    tokens and one more.  ``draft_tokens`` (int32 ``[R - requests]``) holds the requests'
+    drafts one after the other, ``draft_probs [R - requests, V]`` (float32) the distributions
+    they were drawn from; None: drafts that were not drawn (looked up, say), of probability 1.
+
+    With ``p`` the softmax of a row's logits over the temperature, draft ``x`` is taken while
+    ``accept_uniform * q(x) < p(x)``; where one is not, the request's next token is drawn from
+    ``max(p - q, 0)``, behind the last one from ``p``, by the inverse CDF in token order at
+    ``draw_uniform[r]``: tokens come out with the target's own probabilities.  Where
+    ``temperature`` (float32 ``[requests]``) is None or 0, a draft is taken while it is the
+    row's best token and the next token is the best of its row.
+
+    Returns ``(tokens [R], accepted [requests])``, int32: at a request's rows the drafts that
+    were taken, the next token, then -1.  A row with a non-finite logit that the request
+    reaches ends it with -1 in the next token's place."""
+
+    _check(logits, "logits", dtype=torch.float32)
+    if logits.ndim != 2 or logits.numel() == 0:
+        raise KernelError("verify_drafts takes logits [R>0, V>0].")
+    rows, vocab = logits.shape
+    _check(row_start, "row_start", dtype=torch.int32)
+    if row_start.ndim != 1 or not 2 <= row_start.numel() <= rows + 1:
+        raise KernelError(f"verify_drafts: row_start must be [requests + 1] for 1 to {rows} requests.")
+    requests = row_start.numel() - 1
+    _check(draft_tokens, "draft_tokens", dtype=torch.int32, shape=(rows - requests,))
+    if draft_probs is not None:
+        _check(draft_probs, "draft_probs", dtype=torch.float32, shape=(rows - requests, vocab))
+    if temperature is not None:
+        _check(temperature, "temperature", dtype=torch.float32, shape=(requests,))
+        if accept_uniform is None or draw_uniform is None:
+            raise KernelError("verify_drafts: sampling needs uniform numbers.")
+        _check(accept_uniform, "accept_uniform", dtype=torch.float32, shape=(rows - requests,))
+        _check(draw_uniform, "draw_uniform", dtype=torch.float32, shape=(requests,))
+    _check_on_current_device(logits=logits, row_start=row_start, draft_tokens=draft_tokens, draft_probs=draft_probs,
+                             accept_uniform=accept_uniform, draw_uniform=draw_uniform, temperature=temperature)
+    tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    accepted = torch.empty((requests,), dtype=torch.int32, device=logits.device)
+    size = int(load().ms_verify_drafts_workspace_bytes(rows, requests, vocab))
+    workspace = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    # without drafts their tensors are empty, and their addresses null
+    call("ms_verify_drafts", _ptr(logits), _ptr(row_start), _ptr(draft_tokens), _ptr(draft_probs) if rows > requests else None,
+         _ptr(accept_uniform), _ptr(draw_uniform), _ptr(temperature), _ptr(tokens), _ptr(accepted), _ptr(workspace), size,
+         rows, requests, vocab, _stream())
+    return tokens, accepted

@@ -32,6 +32,10 @@ _SIGNATURES: dict[str, list] = {
     "ms_attention_decode_supported": [_I, _I],
     "ms_attention_prefill": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P],
     "ms_attention_prefill_supported": [_I, _I],
+    "ms_attention_shared_prefix": [_P] * 11 + [_I] * 8 + [_F] + [_I] * 5 + [_P],
+    "ms_attention_shared_prefix_supported": [_I, _I],
+    "ms_copy_pages": [_P, _P, _P, _P, _I, _P, _P, _I, _P],
+    "ms_copy_pages_most_pools": [],
     "ms_gemm_f32": [_P, _P, _P, _I, _I, _I, _I, _P],
     "ms_gemm_skinny": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "ms_gemm_skinny_supported": [_I, _I, _I, _I],
@@ -50,6 +54,8 @@ _SIGNATURES: dict[str, list] = {
     "ms_argmax_rows": [_P, _P, _P, _P, _I, _I, _I, _P],
     "ms_sample_rows_workspace_bytes": [_I, _I],
     "ms_sample_rows_chunked": [_P, _P, _P, _P, _P, _P, _P, c_size_t, _I, _I, _I, _P],
+    "ms_verify_drafts": [_P] * 10 + [c_size_t, _I, _I, _I, _P],
+    "ms_verify_drafts_workspace_bytes": [_I, _I, _I],
 }
 
 _lock = threading.Lock()
@@ -72,7 +78,8 @@ def _declare(lib: ctypes.CDLL) -> None:
             ) from None
         function.restype = c_int
         function.argtypes = argtypes
-    lib.ms_sample_rows_workspace_bytes.restype = c_size_t      # a size, not a status
+    lib.ms_sample_rows_workspace_bytes.restype = c_size_t      # sizes, not a status
+    lib.ms_verify_drafts_workspace_bytes.restype = c_size_t
 
 
 def load() -> ctypes.CDLL:
