@@ -1,6 +1,6 @@
 from .allocator import OutOfPagesError, PageAllocator
 from .layout import CacheLayout, CallPlacement, KVGroup
-from .manager import CacheError, CacheManager, CapacitySnapshot, SequenceStepMeta, StepItem, StepReservation
+from .manager import CacheError, CacheManager, CapacitySnapshot, Fork, SequenceStepMeta, StepItem, StepReservation
 from .table import RETURNED, BlockTable
 
 __all__ = [
@@ -10,6 +10,7 @@ __all__ = [
     "CacheManager",
     "CallPlacement",
     "CapacitySnapshot",
+    "Fork",
     "KVGroup",
     "OutOfPagesError",
     "PageAllocator",

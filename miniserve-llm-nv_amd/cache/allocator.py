@@ -54,6 +54,22 @@ class PageAllocator:
             if self._owners[page] == 0:
                 heapq.heappush(self._free, page)
 
+    def move(self, moves: dict[int, int]) -> None:
+        """Held pages get other numbers, ``moves[old] = new``, with the owners they have; the
+        new ones must be free, the old ones are free afterwards."""
+
+        old = self._held(moves.keys(), "move")
+        new = tuple(moves.values())
+        if len(set(new)) != len(new) or any(type(page) is not int or not 0 <= page < self.num_pages for page in new):
+            raise ValueError(f"cannot move pages to {list(new)}: each needs a page of its own in the pool.")
+        if any(self._owners[page] != 0 for page in new):
+            raise RuntimeError(f"cannot move pages to {list(new)}: not all of them are free.")
+        for page, place in moves.items():
+            self._owners[place], self._owners[page] = self._owners[page], 0
+        taken = set(new)
+        self._free = [page for page in self._free if page not in taken] + list(old)
+        heapq.heapify(self._free)
+
     def _held(self, pages: Iterable[int], verb: str) -> tuple[int, ...]:
         """``pages`` as a tuple, after checking all of them (so that a refused call has done nothing)."""
 

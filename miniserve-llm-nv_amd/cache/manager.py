@@ -85,6 +85,14 @@ class StepItem:
     end: int          # length after the step
 
 
+@dataclass(eq=False)
+class Fork:
+    """Requests that were forked from one: the tables of all that still carry this object
+    begin with the same ``pages`` (a number per group)."""
+
+    pages: tuple[int, ...]
+
+
 @dataclass
 class SequenceStepMeta:
     """One request's share of a prepared step."""
@@ -96,6 +104,7 @@ class SequenceStepMeta:
     block_tables: list[tuple[int, ...]]     # per group, committed + tentative pages
     slot_mappings: list[tuple[int, ...]]    # per group, one slot per new token
     new_pages: list[list[int]]              # per group
+    fork: Fork | None = None                # whom the request shares its first pages with
 
 
 @dataclass
@@ -114,6 +123,7 @@ class _Live:
     committed: int = 0
     tables: list[BlockTable] = field(default_factory=list)
     pending: bool = False
+    fork: Fork | None = None
 
 
 class CacheManager:
@@ -272,6 +282,138 @@ class CacheManager:
     def block_table(self, request_id: str, group: int = 0) -> tuple[int, ...]:
         return self._live[request_id].tables[group].snapshot()
 
+    # ---- branches ------------------------------------------------------------------------
+    def _settled(self, request_id: str) -> _Live:
+        live = self._live.get(request_id)
+        if live is None:
+            raise CacheError(f"request {request_id!r} is not live.")
+        if live.pending:
+            raise CacheError(f"request {request_id!r} is part of an open step.")
+        return live
+
+    def _copy_pages(self, group: int, source: Sequence[int], destination: Sequence[int]) -> None:
+        """In every plane and call of the group's pools, in stream order behind the steps that
+        wrote the pages; nothing where no storage is attached."""
+
+        if source and group < len(self.pools):
+            from .. import ops
+
+            ops.copy_pages(list(self.pools[group].values()), source, destination)
+
+    def fork(self, request_id: str, children: Sequence[str]) -> list[int]:
+        """Admit ``children`` as requests that continue where ``request_id`` stands: they hold
+        its whole pages with it, a copy of its last page where that is not full, and a copy
+        of its state.  Returns their state slots.  When slots or pages do not suffice nothing
+        has changed.  (The reference admits every request with an empty table,
+        miniserve/kv/manager.py:81-117; its allocator can count several owners of a page,
+        miniserve/kv/allocator.py:45-62.)"""
+
+        live = self._settled(request_id)
+        children = tuple(children)
+        if len(set(children)) != len(children):
+            raise CacheError(f"a child is named twice in {list(children)}.")
+        for child in children:
+            if child in self._live:
+                raise CacheError(f"request {child!r} is already live.")
+        if len(children) > len(self._free_slots):
+            raise CacheError(f"NO_FREE_SLOT: {len(children)} state slots are needed, {len(self._free_slots)} are free.")
+        if not children:
+            return []
+        whole = tuple(live.committed // size for size in self.block_sizes)
+        last_pages: list[list[int]] = []      # per group, one a child
+        try:
+            for table, allocator, size in zip(live.tables, self.allocators, self.block_sizes):
+                last_pages.append(allocator.allocate(len(children) if live.committed % size else 0))
+            for group, (table, pages) in enumerate(zip(live.tables, last_pages)):
+                if pages:
+                    self._copy_pages(group, [table.pages[whole[group]]] * len(pages), pages)
+        except BaseException:
+            for allocator, pages in zip(self.allocators, last_pages):
+                if pages:
+                    allocator.release(pages)
+            raise
+        fork = Fork(whole) if any(whole) else None
+        live.fork = fork or live.fork
+        slots = []
+        for index, child in enumerate(children):
+            tables = []
+            for table, allocator, count, pages in zip(live.tables, self.allocators, whole, last_pages):
+                forked = table.fork(count)
+                if forked.live_count():
+                    allocator.retain(forked.live_pages())
+                forked.extend(pages[index : index + 1])
+                tables.append(forked)
+            slot = self._free_slots.pop()
+            self._live[child] = _Live(child, slot, committed=live.committed, tables=tables, fork=fork)
+            for tensor in self.state_tensors:
+                tensor[slot].copy_(tensor[live.state_slot])
+            slots.append(slot)
+        return slots
+
+    def truncate(self, request_id: str, length: int) -> None:
+        """Forget the request's tokens from position ``length`` on (drafted tokens that were
+        not taken, say) and give their pages back.  A last page that others hold too is
+        replaced by a copy first, since the next step writes into it.  Refused for a model
+        with state, which cannot be taken back, and where a window's pages that were given
+        back would be needed again.  When a page for a copy is missing nothing has changed."""
+
+        live = self._settled(request_id)
+        if type(length) is not int or not 0 <= length <= live.committed:
+            raise CacheError(f"request {request_id!r} holds {live.committed} tokens, it cannot be cut to {length!r}.")
+        if length == live.committed:
+            return
+        if self.layout.states:
+            raise CacheError("a model with per-request state cannot take tokens back.")
+        copied = []                  # per group: the entry of a page that has to be copied, or None
+        for group, table, allocator, size in zip(self.layout.groups, live.tables, self.allocators, self.block_sizes):
+            if group.window is not None and max(length - group.window + 1, 0) // size < table.first_live:
+                raise CacheError(f"request {request_id!r}: pages that the window of position {length} needs were given back.")
+            entry = length // size if length % size else None
+            if entry is not None and allocator.refcount(table.pages[entry]) == 1:
+                entry = None
+            if entry is not None:
+                dropped = table.pages[table.pages_for(length) :]
+                if allocator.free_count() + sum(allocator.refcount(page) == 1 for page in dropped) == 0:
+                    raise OutOfPagesError(f"request {request_id!r}: no page is free for a copy of a page that others hold.")
+            copied.append(entry)
+        for index, (table, allocator, entry) in enumerate(zip(live.tables, self.allocators, copied)):
+            gone = table.cut(length)
+            if gone:
+                allocator.release(gone)
+            if entry is not None:
+                shared, own = table.pages[entry], allocator.allocate(1)[0]
+                self._copy_pages(index, [shared], [own])
+                table.rename({shared: own})
+                allocator.release([shared])
+        live.committed = length
+        if live.fork is not None and any(length < count * size for count, size in zip(live.fork.pages, self.block_sizes)):
+            live.fork = None
+
+    def compact(self) -> int:
+        """Move pages so that those in use are the first of their pools; returns how many
+        moved.  Not while a step is open."""
+
+        if self._open is not None:
+            raise CacheError("a step is open; pages move between steps.")
+        total = 0
+        for group, allocator in enumerate(self.allocators):
+            used = allocator.used_count()
+            holes = [page for page in allocator.free_ids() if page < used]
+            behind = [page for page in range(used, allocator.num_pages) if allocator.refcount(page) > 0]
+            moves = dict(zip(behind, holes))
+            if moves:
+                self._copy_pages(group, list(moves), list(moves.values()))
+                allocator.move(moves)
+                for live in self._live.values():
+                    live.tables[group].rename(moves)
+            total += len(moves)
+        return total
+
+    def fork_of(self, request_id: str) -> Fork | None:
+        """Whom the request shares its first pages with."""
+
+        return self._live[request_id].fork
+
     # ---- the step transaction ---------------------------------------------------------
     def prepare_step(self, items: Sequence[StepItem]) -> StepReservation:
         if self._open is not None:
@@ -296,7 +438,7 @@ class CacheManager:
         try:
             for item in items:
                 live = self._live[item.request_id]
-                meta = SequenceStepMeta(item.request_id, live.state_slot, item.start, item.end, [], [], [])
+                meta = SequenceStepMeta(item.request_id, live.state_slot, item.start, item.end, [], [], [], live.fork)
                 for index, (allocator, table) in enumerate(zip(self.allocators, live.tables)):
                     missing = table.pages_for(item.end) - len(table.pages)
                     new_pages = allocator.allocate(max(missing, 0))
@@ -397,16 +539,25 @@ class CacheManager:
             free_blocks=tuple(allocator.free_count() for allocator in self.allocators),
             free_slots=len(self._free_slots),
             total_slots=self.max_num_seqs,
-            held_blocks={
-                request_id: tuple(table.live_count() for table in live.tables)
-                for request_id, live in self._live.items()
-            },
+            held_blocks={request_id: self._pages_given_back(live) for request_id, live in self._live.items()},
             windows=tuple(group.window for group in self.layout.groups),
         )
 
+    def _pages_given_back(self, live: _Live) -> tuple[int, ...]:
+        """Pages of each group that come free when the request goes: all it holds, but for
+        those that others hold too."""
+
+        if live.fork is None:
+            return tuple(table.live_count() for table in live.tables)
+        return tuple(
+            sum(allocator.refcount(page) == 1 for page in table.live_pages())
+            for allocator, table in zip(self.allocators, live.tables)
+        )
+
     def assert_invariants(self) -> None:
-        """No page is lost or held twice: per group, the pages of all tables, the
-        open step's tentative pages and the free list are disjoint and add up."""
+        """No page is lost or held by more than own it: per group, every page is in as many
+        tables (the open step's tentative pages counted) as it has owners, once at most in
+        a table, and free where that is none; the tables of a fork begin alike."""
 
         for index, allocator in enumerate(self.allocators):
             allocator.assert_invariants()
@@ -416,12 +567,21 @@ class CacheManager:
             if self._open is not None:
                 for meta in self._open.sequences:
                     held.extend(meta.new_pages[index])
-            if len(held) != len(set(held)):
-                raise AssertionError(f"group {index}: a page is held twice.")
+            times: dict[int, int] = {}
+            for page in held:
+                times[page] = times.get(page, 0) + 1
+            if any(allocator.refcount(page) != count for page, count in times.items()):
+                raise AssertionError(f"group {index}: a page is held twice, or by another number of requests than own it.")
             if set(held) & set(allocator.free_ids()):
                 raise AssertionError(f"group {index}: a held page is on the free list.")
-            if len(held) + allocator.free_count() != allocator.num_pages:
-                raise AssertionError(f"group {index}: pages are lost ({len(held)} held, {allocator.free_count()} free).")
+            if len(times) + allocator.free_count() != allocator.num_pages:
+                raise AssertionError(f"group {index}: pages are lost ({len(times)} held, {allocator.free_count()} free).")
+            fronts: dict[int, list[int]] = {}
+            for live in self._live.values():
+                if live.fork is not None and self.layout.groups[index].window is None:
+                    front = live.tables[index].pages[: live.fork.pages[index]]
+                    if len(front) != live.fork.pages[index] or fronts.setdefault(id(live.fork), front) != front:
+                        raise AssertionError(f"group {index}: tables of a fork do not begin alike.")
         slots = [live.state_slot for live in self._live.values()]
         if len(slots) != len(set(slots)) or set(slots) & set(self._free_slots):
             raise AssertionError("a state slot is held twice.")

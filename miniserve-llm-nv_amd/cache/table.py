@@ -81,6 +81,33 @@ class BlockTable:
             self._tuple = None
         return gone
 
+    def fork(self, whole_pages: int) -> "BlockTable":
+        """Another table over this one's first ``whole_pages`` entries."""
+
+        if not _whole(whole_pages) or whole_pages > len(self.pages):
+            raise ValueError(f"a table of {len(self.pages)} pages cannot be forked after {whole_pages!r}.")
+        other = BlockTable(self.block_size)
+        other.pages = self.pages[:whole_pages]
+        other.first_live = min(self.first_live, whole_pages)
+        return other
+
+    def cut(self, token_count: int) -> list[int]:
+        """The pages wholly behind the first ``token_count`` tokens leave the table and are returned."""
+
+        end = max(self.pages_for(token_count), self.first_live)
+        gone = self.pages[end:]
+        if gone:
+            del self.pages[end:]
+            self._tuple = None
+        return gone
+
+    def rename(self, names: dict[int, int]) -> None:
+        """Pages that were moved inside their pool: ``names[old] = new``."""
+
+        if not names.keys().isdisjoint(self.live_pages()):
+            self.pages[self.first_live :] = [names.get(page, page) for page in self.live_pages()]
+            self._tuple = None
+
     def snapshot(self) -> tuple[int, ...]:
         """The table as a tuple; the same object until the table changes, so a reader
         can tell by identity whether it has seen this table."""

@@ -15,8 +15,8 @@ from typing import Callable, Mapping, Sequence
 import numpy as np
 import torch
 
-from ..cache.manager import StepReservation
-from ..parts.base import GroupStepView, HostBatch, StepContext
+from ..cache.manager import Fork, StepReservation
+from ..parts.base import GroupStepView, HostBatch, SharedFronts, StepContext
 
 
 @dataclass(frozen=True)
@@ -39,6 +39,30 @@ class StepEntry:
             raise ValueError(f"entry {self.request_id!r}: token ids must be non-negative integers.")
         if any(not isinstance(w, int) or isinstance(w, bool) or not 0 <= w < len(self.token_ids) for w in self.want):
             raise ValueError(f"entry {self.request_id!r}: wanted places must index its tokens.")
+
+
+# A step reads common pages of forked requests once (ops.attention_shared_prefix) from this
+# many keys on, and where no request brings more than SHARED_FRONT_TOKENS tokens (a decoded
+# token, or one with drafted ones behind it): prompts go to the tiled kernel.
+SHARED_FRONT_KEYS = 256
+SHARED_FRONT_TOKENS = 16
+
+
+def shared_fronts(forks: Sequence[Fork | None], group: int, block_size: int) -> tuple[list[int], list[int]] | None:
+    """The step's sequences, in the order of its rows, as runs of neighbours of one fork:
+    where each run begins (and the end of the last), and the keys that it shares (0 for a
+    sequence alone).  None when no run shares ``SHARED_FRONT_KEYS``."""
+
+    starts, lens, pays = [0], [], False
+    for row, fork in enumerate(forks):
+        if row > 0 and fork is not None and fork is forks[row - 1]:
+            lens[-1] = fork.pages[group] * block_size
+            pays = pays or lens[-1] >= SHARED_FRONT_KEYS
+            starts[-1] = row + 1
+        else:
+            starts.append(row + 1)
+            lens.append(0)
+    return (starts, lens) if pays else None
 
 
 @dataclass
@@ -116,10 +140,18 @@ def build_step(
     num_rows = sum(len(entry.want) for entry in entries)
     widest = [max(1, max(len(meta.block_tables[group]) for meta in metas_in_layout)) for group in range(num_groups)]
 
+    fronts: list[tuple[list[int], list[int]] | None] = [None] * num_groups
+    forks = [getattr(meta, "fork", None) for meta in metas_in_layout]
+    if any(fork is not None for fork in forks) and max(query_lens) <= SHARED_FRONT_TOKENS:
+        fronts = [shared_fronts(forks, group, block_sizes[group]) for group in range(num_groups)]
+
     offsets: dict[str, tuple[int, int]] = {}
     total = 0
     sizes = [("token_ids", n), ("positions", n), ("seq_of_token", n), ("query_start", s + 1), ("context_lens", s),
              ("state_slots", s), ("logit_rows", num_rows)]
+    for group, front in enumerate(fronts):
+        if front is not None:
+            sizes += [(f"front_start{group}", len(front[0])), (f"front_lens{group}", len(front[1]))]
     sizes += [(f"part:{name}", values.size) for name, values in part_tables.items()]
     for group in range(num_groups):
         sizes += [(f"slots{group}", n), (f"table{group}", s * widest[group])]
@@ -204,14 +236,25 @@ def build_step(
     region("logit_rows")[:] = logit_rows
     for name, values in part_tables.items():
         region(f"part:{name}")[:] = values
+    for group, front in enumerate(fronts):
+        if front is not None:
+            region(f"front_start{group}")[:], region(f"front_lens{group}")[:] = front
     buffer = torch.empty(total, dtype=torch.int32, device=device) if on_gpu else host
 
     def view(name: str) -> torch.Tensor:
         start, length = offsets[name]
         return buffer[start : start + length]
 
+    def shared_view(group: int) -> SharedFronts | None:
+        front = fronts[group]
+        if front is None:
+            return None
+        behind = max(context_lens[row] - length for first, end, length in zip(front[0], front[0][1:], front[1])
+                     for row in range(first, end))
+        return SharedFronts(view(f"front_start{group}"), view(f"front_lens{group}"), max(front[1]), behind, max(query_lens))
+
     groups = [
-        GroupStepView(block_table=view(f"table{g}").view(s, widest[g]), slot_mapping=view(f"slots{g}"))
+        GroupStepView(block_table=view(f"table{g}").view(s, widest[g]), slot_mapping=view(f"slots{g}"), shared=shared_view(g))
         for g in range(num_groups)
     ]
     ctx = StepContext(

@@ -22,8 +22,8 @@ from ..cache import CacheLayout, CacheManager, StepItem
 from ..config import EngineConfig, load_config
 from ..parts.model import TORCH_DTYPES, DecoderModel
 from ..weights import WeightLoadReport, load_weights, random_model_tensors
-from ..parts.base import GroupStepView, HostBatch, StepContext
-from .batch import BuiltStep, StepEntry, build_step
+from ..parts.base import GroupStepView, HostBatch, SharedFronts, StepContext
+from .batch import BuiltStep, StepEntry, build_step, shared_fronts
 
 
 def _require_gpu(device: torch.device) -> None:
@@ -76,11 +76,15 @@ class DecodeGraph:
     token 0 at position 0 of a sequence whose only page is the pools' spare page and
     whose state slot is the spare slot.  They write and read nothing that a request
     holds, and their logits are not returned.
+
+    ``shared``: a recording for steps with neighbouring rows of forked requests; where those
+    runs lie and how many keys they share is among the step's numbers.
     """
 
-    def __init__(self, runner: "ModelRunner", batch: int, bound: int) -> None:
+    def __init__(self, runner: "ModelRunner", batch: int, bound: int, shared: bool = False) -> None:
         self.batch = batch
         self.bound = bound
+        self.shared = shared
         # no strong reference back: a runner that is dropped goes at once, with its graphs,
         # and not at some later collection of cycles
         self._runner = weakref.ref(runner)
@@ -95,6 +99,8 @@ class DecodeGraph:
         sizes += [(f"part:{name}", values.size) for name, values in part_tables.items()]
         for group in range(groups):
             sizes += [(f"slots{group}", batch), (f"table{group}", batch * widths[group])]
+            if shared:
+                sizes += [(f"front_start{group}", batch + 1), (f"front_lens{group}", batch)]
         # for a step launched behind the sampling of the step before: which of that step's rows each row continues
         sizes += [("token_rows", batch)]
         self.offsets: dict[str, tuple[int, int]] = {}
@@ -124,7 +130,8 @@ class DecodeGraph:
             context_lens=view("context_lens"),
             state_slots=view("state_slots"),
             groups=[
-                GroupStepView(block_table=view(f"table{g}").view(batch, widths[g]), slot_mapping=view(f"slots{g}"))
+                GroupStepView(block_table=view(f"table{g}").view(batch, widths[g]), slot_mapping=view(f"slots{g}"),
+                              shared=SharedFronts(view(f"front_start{g}"), view(f"front_lens{g}"), bound, bound, 1) if shared else None)
                 for g in range(groups)
             ],
             # what holds for every replay: one token a row.  Launch decisions inside the
@@ -174,7 +181,13 @@ class DecodeGraph:
         put("context_lens", [meta.after for meta in metas] + [1] * spare)
         put("state_slots", [meta.state_slot for meta in metas] + [runner.cache.spare_state_slot] * spare)
         put("logit_rows", range(batch))
+        forks = [meta.fork for meta in metas]
         for group in range(len(runner.cache.layout.groups)):
+            if self.shared:
+                # rows in no run, and runs that are not there, share nothing
+                starts, lens = shared_fronts(forks, group, runner.cache.block_sizes[group]) or ([0], [])
+                put(f"front_start{group}", starts + [starts[-1]] * (batch + 1 - len(starts)))
+                put(f"front_lens{group}", lens + [0] * (batch - len(lens)))
             pool_pages = runner.cache.num_blocks[group]
             block_size, width = runner.cache.block_sizes[group], self.widths[group]
             slots = []
@@ -341,7 +354,7 @@ class ModelRunner:
         )
         self.cache.allocate_storage(self.dtype, self.device)
         self._call_views = self.cache.call_views()
-        self._decode_graphs: dict[tuple[int, int], DecodeGraph] = {}     # by (rows, context bound)
+        self._decode_graphs: dict[tuple, DecodeGraph] = {}     # by (rows, context bound), and True for steps with shared fronts
         self._graph_pool = None
         self.steps_run = 0
         self.tokens_run = 0
@@ -397,11 +410,23 @@ class ModelRunner:
         blocks = max(1, min(by_memory, by_need))
         return blocks
 
-    def _recorded_step_key(self, batch: int, longest: int) -> tuple[int, int]:
-        """(rows, context bound) of the recorded step that serves ``batch`` single tokens
-        whose longest row has ``longest`` tokens after the step."""
+    def _recorded_step_key(self, longest: int, forks: Sequence) -> tuple:
+        """(rows, context bound) of the recorded step that serves a single token for each of
+        ``forks`` (the requests' ``Fork`` or None), the longest row of which has ``longest``
+        tokens after the step; with True behind them for a step that reads common pages of
+        neighbouring rows once."""
 
-        return recorded_batch_size(batch), recorded_context_bound(longest, self.max_model_len)
+        key = recorded_batch_size(len(forks)), recorded_context_bound(longest, self.max_model_len)
+        if self.dtype == torch.bfloat16 and any(fork is not None for fork in forks) and any(
+            group.window is None and shared_fronts(forks, group.index, self.cache.block_sizes[group.index])
+            for group in self.cache.layout.groups
+        ):
+            key += (True,)
+        return key
+
+    def _recorded_step_key_of(self, reservation) -> tuple:
+        metas = reservation.sequences
+        return self._recorded_step_key(max(meta.after for meta in metas), [meta.fork for meta in metas])
 
     def _decode_graph_step(self, entries: Sequence[StepEntry], reservation, prepared: int | None = None) -> torch.Tensor | None:
         """A step of single tokens through the recorded graph of its batch size.  The
@@ -411,7 +436,7 @@ class ModelRunner:
             if entry.token_ids[0] >= self.spec.vocab_size:
                 raise ValueError(f"entry {entry.request_id!r}: a token id is outside the vocabulary.")
         batch = len(entries)
-        key = self._recorded_step_key(batch, max(meta.after for meta in reservation.sequences))
+        key = self._recorded_step_key_of(reservation)
         graph = self._decode_graphs.get(key)
         if graph is None:
             if self._graph_pool is None:
@@ -432,6 +457,27 @@ class ModelRunner:
     def release(self, request_id: str) -> None:
         self.cache.release(request_id)
 
+    @torch.inference_mode()
+    def fork(self, request_id: str, children: Sequence[str]) -> list[int]:
+        """Admit ``children`` as branches of ``request_id``: their next step continues behind
+        the tokens that it has run.  They share its full pages, which steps with neighbouring
+        branches read once (:func:`ops.attention_shared_prefix`)."""
+
+        return self.cache.fork(request_id, children)
+
+    @torch.inference_mode()
+    def truncate(self, request_id: str, length: int) -> None:
+        """Forget the request's tokens behind the first ``length``: drafted tokens that were
+        run by a step and not taken (``Sampler.stage_drafts``)."""
+
+        self.cache.truncate(request_id, length)
+
+    @torch.inference_mode()
+    def compact(self) -> int:
+        """Move the pages in use to the front of their pools; returns how many moved."""
+
+        return self.cache.compact()
+
     # ---- the step ---------------------------------------------------------------------
     def prepare_decode(self, request_ids: Sequence[str]) -> "PreparedDecode | None":
         """Opens the cache transaction of a coming step in which each of these requests
@@ -447,7 +493,8 @@ class ModelRunner:
         for request_id in request_ids:
             start = self.cache.committed_tokens(request_id)
             items.append(StepItem(request_id, start, start + 1))
-        graph = self._decode_graphs.get(self._recorded_step_key(len(items), max(item.end for item in items)))
+        graph = self._decode_graphs.get(self._recorded_step_key(
+            max(item.end for item in items), [self.cache.fork_of(request_id) for request_id in request_ids]))
         if graph is None or graph.graph is None:
             return None
         reservation = self.cache.prepare_step(items)
@@ -506,7 +553,7 @@ class ModelRunner:
         elif len(source_rows) != rows or any(not 0 <= row < tokens.numel() for row in source_rows):
             raise ValueError("a chained step's row map names one row of the tokens for each of its requests.")
         metas = prepared.reservation.sequences
-        graph = self._decode_graphs[self._recorded_step_key(len(metas), max(meta.after for meta in metas))]
+        graph = self._decode_graphs[self._recorded_step_key_of(prepared.reservation)]
         graph.launch_chained(prepared.buffer, tokens, len(metas), source_rows)
         prepared.launched = True
         self.chained_steps += 1
@@ -553,8 +600,7 @@ class ModelRunner:
             reservation = self._open_step(entries)
         if prepared is not None and prepared.launched:
             # the step runs already (launch_chained): its logits lie in its recording's output
-            metas = reservation.sequences
-            graph = self._decode_graphs[self._recorded_step_key(len(metas), max(meta.after for meta in metas))]
+            graph = self._decode_graphs[self._recorded_step_key_of(reservation)]
             self.cache.commit_step(reservation)
             self.steps_run += 1
             self.tokens_run += len(entries)

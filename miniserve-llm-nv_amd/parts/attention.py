@@ -167,19 +167,38 @@ class Attention(Part):
             )
         else:
             q = self._prepare_unfused(packed, ctx, cache, group, kv_heads)
-        attended = ops.attention(
-            q,
-            cache.key,
-            cache.value,
-            block_table=group.block_table,
-            seq_of_token=ctx.seq_of_token,
-            positions=ctx.positions,
-            scale=self.scale,
-            window=self.window,
-            decode_prefix=ctx.decode_prefix,
-            tiles=self._tiles(ctx),
-            max_context=ctx.max_context_len,
-        )
+        shared = group.shared
+        # (a 32-bit result must not hang on what else is in the batch, so each sequence reads its own keys there)
+        if (shared is not None and self.window is None and q.dtype == torch.bfloat16
+                and ops.can_share_prefix(self.head_dim, cache.block_size)):
+            attended = ops.attention_shared_prefix(
+                q,
+                cache.key,
+                cache.value,
+                block_table=group.block_table,
+                query_start=ctx.query_start,
+                context_lens=ctx.context_lens,
+                group_start=shared.group_start,
+                shared_lens=shared.shared_lens,
+                scale=self.scale,
+                max_shared=shared.max_shared,
+                max_own=shared.max_own,
+                max_query=shared.max_query,
+            )
+        else:
+            attended = ops.attention(
+                q,
+                cache.key,
+                cache.value,
+                block_table=group.block_table,
+                seq_of_token=ctx.seq_of_token,
+                positions=ctx.positions,
+                scale=self.scale,
+                window=self.window,
+                decode_prefix=ctx.decode_prefix,
+                tiles=self._tiles(ctx),
+                max_context=ctx.max_context_len,
+            )
         attended = attended.reshape(n, self.num_heads * self.head_dim)
         return add_output(attended, self.w_o, residual, norm_after)
 

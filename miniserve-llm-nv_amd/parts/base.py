@@ -152,11 +152,25 @@ class StateView:
 # ---- the batch of one step, as parts see it ---------------------------------------
 
 @dataclass
+class SharedFronts:
+    """Runs of neighbouring sequences whose block tables begin with the same pages: group
+    ``g`` is the sequences ``group_start[g] .. group_start[g + 1] - 1``, which share their
+    first ``shared_lens[g]`` keys.  The bounds hold for every replay of a recorded step."""
+
+    group_start: torch.Tensor    # int32 [groups + 1]
+    shared_lens: torch.Tensor    # int32 [groups]
+    max_shared: int
+    max_own: int                 # keys behind the shared ones
+    max_query: int               # tokens that a sequence brings
+
+
+@dataclass
 class GroupStepView:
     """Cache metadata of one group for this step."""
 
     block_table: torch.Tensor    # int32 [S, max_blocks]
     slot_mapping: torch.Tensor   # int32 [N]: page * block_size + offset of each new token
+    shared: SharedFronts | None = None    # where forked requests stand side by side and it pays to read their common pages once
 
 
 @dataclass(frozen=True)

@@ -1,3 +1,3 @@
-from .sampler import NonFiniteLogitsError, Sampler, StagedSample
+from .sampler import NonFiniteLogitsError, Sampler, StagedDrafts, StagedSample
 
-__all__ = ["NonFiniteLogitsError", "Sampler", "StagedSample"]
+__all__ = ["NonFiniteLogitsError", "Sampler", "StagedDrafts", "StagedSample"]

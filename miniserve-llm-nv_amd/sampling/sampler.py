@@ -29,6 +29,14 @@ class StagedSample:
     generator_state: torch.Tensor | None      # None: greedy, no randomness used
 
 
+@dataclass(frozen=True)
+class StagedDrafts:
+    request_id: str
+    token_ids: tuple[int, ...]                # the drafted tokens that were taken, then one more
+    accepted: int                             # how many of the drafted tokens were taken
+    generator_state: torch.Tensor | None      # None: greedy, no randomness used
+
+
 class NonFiniteLogitsError(ValueError):
     pass
 
@@ -144,7 +152,71 @@ class Sampler:
             for (request_id, _), token, state in zip(requests, token_ids, states)
         )
 
-    def commit(self, samples: Sequence[StagedSample]) -> None:
+    def stage_drafts(
+        self,
+        logits: torch.Tensor,
+        requests: Sequence[tuple[str, SamplingParams, Sequence[int]]],
+        draft_probs: torch.Tensor | None = None,
+    ) -> tuple[StagedDrafts, ...]:
+        """Which of each request's drafted tokens the model takes, and the token behind them:
+        ``logits`` (float32, on the GPU) holds for each request the rows of its drafted
+        tokens' places and one more, as a step gives them whose entry brings the last token
+        and the drafted ones and wants all of their places.  ``draft_probs``: the
+        distributions that the drafted tokens were drawn from, a row each; None: they were
+        not drawn.  Tokens come out with the probabilities that sampling one at a time would
+        give them (greedy: they are the same tokens).  A request draws one uniform number a
+        drafted token and one for the token behind; as with :meth:`stage` its generator
+        advances at :meth:`commit`."""
+
+        from .. import ops
+
+        for request_id, params, drafts in requests:
+            if params.temperature > 0 and (params.top_k != 0 or params.top_p < 1):
+                raise ValueError(f"request {request_id!r}: drafted tokens are compared with whole distributions, without top-k and top-p.")
+            if any(type(token) is not int or token < 0 for token in drafts):
+                raise ValueError(f"request {request_id!r}: drafted tokens must be non-negative integers.")
+        counts = [len(drafts) for _, _, drafts in requests]
+        rows, drafted = sum(counts) + len(requests), sum(counts)
+        if not requests or logits.ndim != 2 or logits.shape[0] != rows:
+            raise ValueError(f"{len(requests)} requests with {drafted} drafted tokens need {rows} rows of logits, not {tuple(logits.shape)}.")
+        states: list[torch.Tensor | None] = []
+        accept: list[float] = []
+        draw: list[float] = []
+        for request_id, params, drafts in requests:
+            if params.temperature == 0:
+                states.append(None)
+                accept += [0.0] * len(drafts)
+                draw.append(0.0)
+                continue
+            scratch = torch.Generator(device="cpu")
+            scratch.set_state((self._generators.get(request_id) or self._new_generator(params)).get_state())
+            accept += [self.draw_uniform(scratch) for _ in drafts]
+            draw.append(self.draw_uniform(scratch))
+            states.append(scratch.get_state())
+        # all numbers in one pinned buffer and one copy
+        sizes = [len(requests) + 1, drafted, drafted, len(requests), len(requests)]
+        host = torch.empty(sum(sizes), dtype=torch.float32, pin_memory=logits.is_cuda)
+        starts = np.concatenate(([0], np.cumsum([count + 1 for count in counts])))
+        numbers = [part.numpy() for part in host.split(sizes)]
+        numbers[0].view(np.int32)[:] = starts
+        numbers[1].view(np.int32)[:] = [token for _, _, drafts in requests for token in drafts]
+        numbers[2][:], numbers[3][:] = accept, draw
+        numbers[4][:] = [params.temperature for _, params, _ in requests]
+        sent = host.to(logits.device, non_blocking=True).split(sizes)
+        tokens, accepted = ops.verify_drafts(
+            logits.float().contiguous(), sent[0].view(torch.int32), sent[1].view(torch.int32), draft_probs=draft_probs,
+            accept_uniform=sent[2], draw_uniform=sent[3], temperature=sent[4],
+        )
+        chosen = torch.cat([tokens, accepted]).tolist()
+        staged = []
+        for (request_id, _, _), first, taken, state in zip(requests, starts.tolist(), chosen[rows:], states):
+            ids = tuple(chosen[first : first + taken + 1])
+            if ids[-1] < 0:
+                raise NonFiniteLogitsError("a row of logits holds a value that is not finite; no token can be chosen from it.")
+            staged.append(StagedDrafts(request_id, ids, taken, state))
+        return tuple(staged)
+
+    def commit(self, samples: Sequence[StagedSample | StagedDrafts]) -> None:
         for sample in samples:
             if sample.generator_state is None:
                 continue
