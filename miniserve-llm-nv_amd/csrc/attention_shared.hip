@@ -11,13 +11,19 @@
 // The parts here are splits of the group's shared keys and splits of the sequence's own
 // keys behind them.  One kernel makes the (m, l, O) of all parts, a second joins them.
 //
-// A workgroup of 4 waves takes a tile of 16 R rows of one kv head (rows of the whole
-// group for shared keys, of one sequence for its own) and a range of keys, which its waves
-// walk in pairs of 16-key tiles, each wave pairs of its own, with its own running maximum,
-// sum and output (32-bit); they are joined through LDS at the end.  Operands come from the
-// cache as it lies (see attention_tiles.hpp); 32-bit storage runs the same walk on the
-// 32-bit matrix instruction.
-#include "mfma.hpp"
+// A workgroup takes a tile of rows of one kv head (rows of the whole group for
+// shared keys, of one sequence for its own) and a range of keys, dealt out to the waves in
+// pairs of 16-key tiles.  Two walks:
+//
+//   direct   tiles of 16 or 32 rows, 16x16x32 products, every wave against pairs of its own,
+//            operands from the cache straight into registers (few rows: the keys' bytes
+//            are what it costs).  32-bit storage runs it on the 32-bit matrix instruction.
+//   columns  tiles of 64 or 128 rows, 32x32x16 products, 32 rows to a wave: the waves of a
+//            part share every pair through LDS (many rows: each key read from the L2 has
+//            to serve as many of them as possible).
+//
+// The waves' (m, l, O) are joined through LDS, so a workgroup leaves one part a row.
+#include "attention_columns.hpp"
 
 namespace {
 
@@ -28,10 +34,19 @@ using ms::floatx4;
 
 typedef float floatx8 __attribute__((ext_vector_type(8)));
 
-constexpr int kTileKeys = 16;
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * ms::kWave;
+using ms::kTileKeys;
+
+constexpr int kXcds = 8;            // dies of the chip, each with an L2 of its own (a wrong number costs speed only)
+// Waves of a workgroup by the rows of its tile.  A compute unit holds eight of these waves
+// (registers), and draws some 50 GB/s from memory whatever they have under way.  Few rows
+// are bound by that and by the chain of loads at a workgroup's start: two workgroups of
+// four waves, so that one's start runs beside the other's walk, and the keys on as many
+// units as there are.  Many rows want one workgroup whose waves share every key.
+constexpr int waves_of(int rows) { return rows <= 32 ? 4 : 8; }
 constexpr int kMaxSplits = 64;      // of the shared keys, and of a sequence's own
+// Fewest keys of a split (but for the last): a pair of tiles for every wave.  A shorter one
+// leaves waves idle and gives the join more parts.
+constexpr int split_keys(int rows) { return 2 * kTileKeys * waves_of(rows); }
 
 // ---- operands by storage type -------------------------------------------------------
 
@@ -97,13 +112,14 @@ struct Batch {
   const int32_t* __restrict__ shared_lens;
   int num_tokens, num_seqs, num_groups, num_q_heads, num_kv_heads, block_size, max_blocks;
   float scale;
-  int shared_tiles, shared_splits, own_tiles, own_splits;
+  int tile_rows, shared_tiles, shared_splits, own_tiles, own_splits;
 };
 
 // Rows and keys of one workgroup, the same in all its lanes.
 struct Work {
   int first_token;        // of the rows' segment (a group's or a sequence's tokens, which are contiguous)
   int rows, row0;         // rows of the segment, first row of this tile
+  int kv_head;
   int first_key, end_key;         // keys [first_key, end_key) of this split
   int pos_of_first;       // row of token i sees keys <= pos_of_first + i; for shared keys every row sees all
   bool causal;
@@ -112,8 +128,8 @@ struct Work {
 };
 
 // The group's part of a flat list of tiles: every group has ceil(rows / tile_rows) of them.
-__device__ __forceinline__ bool find_group_tile(const Batch& b, int tile, int group_rows_per_token, int tile_rows,
-                                                int& group, int& local) {
+__device__ __forceinline__ bool find_group_tile(const Batch& b, int tile, int rows_per_token, int tile_rows, int& group,
+                                                int& local) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int g0 = 0; g0 < b.num_groups; g0 += ms::kWave) {
@@ -121,7 +137,7 @@ __device__ __forceinline__ bool find_group_tile(const Batch& b, int tile, int gr
     int tiles = 0;
     if (g < b.num_groups) {
       const int tokens = b.query_start[b.group_start[g + 1]] - b.query_start[b.group_start[g]];
-      tiles = (tokens * group_rows_per_token + tile_rows - 1) / tile_rows;
+      tiles = (tokens * rows_per_token + tile_rows - 1) / tile_rows;
     }
     int upto = tiles;
 #pragma unroll
@@ -139,6 +155,17 @@ __device__ __forceinline__ bool find_group_tile(const Batch& b, int tile, int gr
     base += __shfl(upto, ms::kWave - 1, ms::kWave);
   }
   return false;
+}
+
+// The most keys that a group shares.  Splits are cut by it, so that those of all groups
+// have the same number of keys (a short group has fewer of them).
+__device__ __forceinline__ int longest_shared(const Batch& b) {
+  const int lane = threadIdx.x & 63;
+  int longest = 0;
+  for (int g = lane; g < b.num_groups; g += ms::kWave) longest = max(longest, b.shared_lens[g]);
+#pragma unroll
+  for (int offset = 32; offset > 0; offset >>= 1) longest = max(longest, __shfl_xor(longest, offset, ms::kWave));
+  return ms::uniform(longest);
 }
 
 // The group of a sequence, -1 for one that is in none.
@@ -163,32 +190,31 @@ struct Pair {
   typename Operand<T>::V4 v_a[CS], v_b[CS];
 };
 
+// ``pages``: of the pair's two tiles, looked up a round earlier.
 template <typename T, int D>
-__device__ __forceinline__ void load_pair(Pair<T, D>& pair, const Batch& b, const Work& w, int tile, int last_tile,
+__device__ __forceinline__ void load_pair(Pair<T, D>& pair, const Batch& b, const ms::PairPages& pages,
                                           const T* __restrict__ key_pool, const T* __restrict__ value_pool, int kv_head,
                                           int g, int r) {
+  // bases that are the same in all lanes, and 32-bit lane offsets that never change
   using Op = Operand<T>;
-  const int key_a = tile * kTileKeys;
-  const int key_b = min(tile + 1, last_tile) * kTileKeys;       // without a second tile the first is read twice
-  const int page_a = key_a / b.block_size, page_b = key_b / b.block_size;
-  const int off_a = key_a - page_a * b.block_size, off_b = key_b - page_b * b.block_size;
-  const int64_t slab_a = static_cast<int64_t>(w.table[page_a]) * b.num_kv_heads + kv_head;
-  const int64_t slab_b = static_cast<int64_t>(w.table[page_b]) * b.num_kv_heads + kv_head;
-  const T* k_row_a = key_pool + (slab_a * b.block_size + off_a + r) * D;
-  const T* k_row_b = key_pool + (slab_b * b.block_size + off_b + r) * D;
-  const T* v_a = value_pool + slab_a * D * b.block_size + off_a + 4 * g;
-  const T* v_b = value_pool + slab_b * D * b.block_size + off_b + 4 * g;
+  const int64_t page_stride = static_cast<int64_t>(b.num_kv_heads) * b.block_size * D;
+  const int head_base = kv_head * b.block_size * D;
+  const T* k_a = key_pool + (pages.page[0] * page_stride + head_base + pages.offset[0] * D);
+  const T* k_b = key_pool + (pages.page[1] * page_stride + head_base + pages.offset[1] * D);
+  const T* v_a = value_pool + (pages.page[0] * page_stride + head_base + pages.offset[0]);
+  const T* v_b = value_pool + (pages.page[1] * page_stride + head_base + pages.offset[1]);
+  const uint32_t k_lane = r * D + 8 * g, v_lane = r * b.block_size + 4 * g;
 #pragma unroll
   for (int s = 0; s < Pair<T, D>::KS; ++s) {
-    const int d0 = 32 * s + 8 * g;
-    pair.k_a[s] = d0 < D ? *reinterpret_cast<const typename Op::V8*>(k_row_a + d0) : Op::zero8();
-    pair.k_b[s] = d0 < D ? *reinterpret_cast<const typename Op::V8*>(k_row_b + d0) : Op::zero8();
+    // (a head size off the grid of 32: the last slice's upper half lies in no row)
+    const bool inside = D % 32 == 0 || s + 1 < Pair<T, D>::KS || g < 2;
+    pair.k_a[s] = inside ? *reinterpret_cast<const typename Op::V8*>(k_a + 32 * s + k_lane) : Op::zero8();
+    pair.k_b[s] = inside ? *reinterpret_cast<const typename Op::V8*>(k_b + 32 * s + k_lane) : Op::zero8();
   }
 #pragma unroll
   for (int c = 0; c < Pair<T, D>::CS; ++c) {
-    const int64_t d = 16 * c + r;
-    pair.v_a[c] = *reinterpret_cast<const typename Op::V4*>(v_a + d * b.block_size);
-    pair.v_b[c] = *reinterpret_cast<const typename Op::V4*>(v_b + d * b.block_size);
+    pair.v_a[c] = *reinterpret_cast<const typename Op::V4*>(v_a + 16 * c * b.block_size + v_lane);
+    pair.v_b[c] = *reinterpret_cast<const typename Op::V4*>(v_b + 16 * c * b.block_size + v_lane);
   }
 }
 
@@ -246,27 +272,54 @@ __device__ __forceinline__ void consume(RowState<D>& st, const Pair<T, D>& pair,
   }
 }
 
-// 16 R rows against the keys of ``w``; leaves (m, l, O) of the part in the rows' slots.
-template <typename T, int D, int R>
-__device__ void walk(const Batch& b, const Work& w, const T* __restrict__ q, const T* __restrict__ key_pool,
-                     const T* __restrict__ value_pool, float* __restrict__ partial_o, float* __restrict__ partial_ml,
-                     float* __restrict__ lds) {
+// Values of keys outside the range may never have been written: they must not meet a zero weight.
+template <typename T, int D>
+__device__ __forceinline__ void clear_outside(Pair<T, D>& pair, int tile, int first_key, int end_key, int g) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int ka = tile * kTileKeys + 4 * g + e, kb = ka + kTileKeys;
+#pragma unroll
+    for (int c = 0; c < Pair<T, D>::CS; ++c) {
+      if (ka < first_key || ka >= end_key) Operand<T>::clear(pair.v_a[c], e);
+      if (kb < first_key || kb >= end_key) Operand<T>::clear(pair.v_b[c], e);
+    }
+  }
+}
+
+__device__ __forceinline__ int64_t slot_of(const Batch& b, const Work& w, int row) {
+  const int per_token = b.num_q_heads / b.num_kv_heads;
+  const int token = row / per_token, head = w.kv_head * per_token + row - token * per_token;
+  return (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * (b.shared_splits + b.own_splits) + w.slot;
+}
+
+// Rows of outputs in LDS are padded by four values, so that the four rows that a wave stores
+// at once lie in different banks.
+template <int D, int WAVES>
+constexpr size_t direct_lds_bytes() {
+  return (2 * WAVES * 16 + WAVES * 16 * (D + 4)) * sizeof(float);
+}
+
+// 16 R rows against the keys of ``w`` (at least one), by the wave's pairs: every WAVES-th.
+template <typename T, int D, int R, int WAVES>
+__device__ __forceinline__ void walk_rows(RowState<D> (&st)[R], const Batch& b, const Work& w, const T* __restrict__ q,
+                                          const T* __restrict__ key_pool, const T* __restrict__ value_pool, int wave) {
   using Op = Operand<T>;
   constexpr int KS = Pair<T, D>::KS, CS = D / 16;
   const int lane = threadIdx.x & 63;
-  const int wave = ms::uniform(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int kv_head = blockIdx.y;
   const int per_token = b.num_q_heads / b.num_kv_heads;
-  const int slots = b.shared_splits + b.own_splits;
+  const int end_tile = (w.end_key - 1) / kTileKeys + 1;
+  constexpr int step = 2 * WAVES;
+  int t = w.first_key / kTileKeys + 2 * wave;
+  // (a pair behind the end is looked up as the last one, and not loaded)
+  ms::PairPages pages = ms::find_pair_pages(t, end_tile, w.table, b.block_size);
 
   typename Op::V8 q_reg[R][KS];
   int last[R];
-  RowState<D> st[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = w.row0 + 16 * i + r;
-    const int token = row / per_token, head = kv_head * per_token + row % per_token;
+    const int token = row / per_token, head = w.kv_head * per_token + row - token * per_token;
     const bool live = row < w.rows;
     last[i] = !live ? -1 : w.causal ? min(w.end_key - 1, w.pos_of_first + token) : w.end_key - 1;
     const T* q_row = q + (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * D;
@@ -281,33 +334,67 @@ __device__ void walk(const Batch& b, const Work& w, const T* __restrict__ q, con
     st[i].run_sum = 0.f;
   }
 
-  if (w.first_key < w.end_key) {
-    const int first_tile = w.first_key / kTileKeys, last_tile = (w.end_key - 1) / kTileKeys;
-    for (int t = first_tile + 2 * wave; t <= last_tile; t += 2 * kWaves) {
-      Pair<T, D> pair;
-      load_pair<T, D>(pair, b, w, t, last_tile, key_pool, value_pool, kv_head, g, r);
-      if (t * kTileKeys < w.first_key || (t + 2) * kTileKeys > w.end_key) {
-        // keys outside the range may never have been written: their values must not meet a zero weight
+  const auto consume_all = [&](Pair<T, D>& pair, int tile) {
+    if (tile * kTileKeys < w.first_key || (tile + 2) * kTileKeys > w.end_key)
+      clear_outside<T, D>(pair, tile, w.first_key, w.end_key, g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int ka = t * kTileKeys + 4 * g + e, kb = ka + kTileKeys;
-#pragma unroll
-          for (int c = 0; c < CS; ++c) {
-            if (ka < w.first_key || ka >= w.end_key) Op::clear(pair.v_a[c], e);
-            if (kb < w.first_key || kb >= w.end_key) Op::clear(pair.v_b[c], e);
-          }
+    for (int i = 0; i < R; ++i) consume<T, D>(st[i], pair, q_reg[i], tile, w.first_key, last[i], b.scale * Op::kScale, g);
+  };
+  // One pair on its way while another is consumed, where the registers hold two.
+  constexpr bool kAhead = R == 1 && sizeof(T) == 2;
+  if constexpr (kAhead) {
+    if (t < end_tile) {
+      Pair<T, D> ping, pong;
+      load_pair<T, D>(ping, b, pages, key_pool, value_pool, w.kv_head, g, r);
+      pages = ms::find_pair_pages(t + step, end_tile, w.table, b.block_size);
+      while (true) {
+        int next = t + step;
+        if (next < end_tile) {
+          load_pair<T, D>(pong, b, pages, key_pool, value_pool, w.kv_head, g, r);
+          pages = ms::find_pair_pages(next + step, end_tile, w.table, b.block_size);
         }
+        consume_all(ping, t);
+        t = next;
+        if (t >= end_tile) break;
+        next = t + step;
+        if (next < end_tile) {
+          load_pair<T, D>(ping, b, pages, key_pool, value_pool, w.kv_head, g, r);
+          pages = ms::find_pair_pages(next + step, end_tile, w.table, b.block_size);
+        }
+        consume_all(pong, t);
+        t = next;
+        if (t >= end_tile) break;
       }
-#pragma unroll
-      for (int i = 0; i < R; ++i)
-        consume<T, D>(st[i], pair, q_reg[i], t, w.first_key, last[i], b.scale * Op::kScale, g);
+    }
+  } else {
+    for (; t < end_tile; t += step) {
+      Pair<T, D> pair;
+      load_pair<T, D>(pair, b, pages, key_pool, value_pool, w.kv_head, g, r);
+      pages = ms::find_pair_pages(t + step, end_tile, w.table, b.block_size);
+      consume_all(pair, t);
     }
   }
+}
 
-  // ---- the waves' states, joined 16 rows at a time -------------------------------------
-  float* m_s = lds;                                  // [kWaves][16]
-  float* l_s = m_s + kWaves * 16;                    // [kWaves][16]
-  float* o_s = l_s + kWaves * 16;                    // [kWaves - 1][16][D]
+// 16 R rows by the whole workgroup: the pairs dealt out to the waves, their states joined
+// through LDS, 16 rows at a time, four values of a row to a thread.
+template <typename T, int D, int R, int WAVES>
+__device__ __forceinline__ void walk_direct(const Batch& b, const Work& w, const T* __restrict__ q,
+                                            const T* __restrict__ key_pool, const T* __restrict__ value_pool,
+                                            float* __restrict__ partial_o, float* __restrict__ partial_ml,
+                                            float* __restrict__ lds) {
+  using Op = Operand<T>;
+  constexpr int CS = D / 16, ROW = D + 4;
+  const int lane = threadIdx.x & 63;
+  const int wave = ms::uniform(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  RowState<D> st[R];
+  walk_rows<T, D, R, WAVES>(st, b, w, q, key_pool, value_pool, wave);
+  float* m_s = lds;                                  // [WAVES][16]
+  float* l_s = m_s + WAVES * 16;                    // [WAVES][16]
+  float* o_s = l_s + WAVES * 16;                    // [WAVES][16][ROW]
+  constexpr int kAtOnce = WAVES * ms::kWave / (D / 4);      // rows that the threads finish at once
+  const int first_row = threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (i > 0) __syncthreads();
@@ -315,133 +402,306 @@ __device__ void walk(const Batch& b, const Work& w, const T* __restrict__ q, con
       m_s[wave * 16 + r] = st[i].run_max;
       l_s[wave * 16 + r] = st[i].run_sum;
     }
-    if (wave > 0) {
 #pragma unroll
-      for (int c = 0; c < CS; ++c)
+    for (int c = 0; c < CS; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o_s[((wave - 1) * 16 + 4 * g + e) * D + 16 * c + r] = st[i].o[c][e];
-    }
+      for (int e = 0; e < 4; ++e) o_s[(wave * 16 + 4 * g + e) * ROW + 16 * c + r] = st[i].o[c][e];
     __syncthreads();
-    if (wave != 0) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int in_tile = 4 * g + e;
-      const int row = w.row0 + 16 * i + in_tile;
-      if (row >= w.rows) continue;
+    if (first_row >= kAtOnce) continue;                     // threads that are left over
+#pragma unroll 1
+    for (int in_tile = first_row; in_tile < 16 && w.row0 + 16 * i + in_tile < w.rows; in_tile += kAtOnce) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) mx = fmaxf(mx, m_s[v * 16 + in_tile]);
+      for (int v = 0; v < WAVES; ++v) mx = fmaxf(mx, m_s[v * 16 + in_tile]);
       const float shift = mx == -INFINITY ? 0.f : mx;
-      float factor[kWaves], sum = 0.f;
+      float sum = 0.f;
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
+      for (int v = 0; v < WAVES; ++v) {
         // 0 for a wave without keys; a NaN among its scores stays one in its sum
-        factor[v] = Op::weight(m_s[v * 16 + in_tile] - shift);
-        sum += factor[v] * l_s[v * 16 + in_tile];
+        const float factor = Op::weight(m_s[v * 16 + in_tile] - shift);
+        const floatx4 o = *reinterpret_cast<const floatx4*>(&o_s[(v * 16 + in_tile) * ROW + d]);
+        sum += factor * l_s[v * 16 + in_tile];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], factor, acc[e]);
       }
-      const int token = row / per_token, head = kv_head * per_token + row % per_token;
-      const int64_t slot = (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * slots + w.slot;
-      if (r == 0) {
+      const int64_t slot = slot_of(b, w, w.row0 + 16 * i + in_tile);
+      if (d == 0) {
         partial_ml[2 * slot] = mx;
         partial_ml[2 * slot + 1] = sum;
       }
-#pragma unroll
-      for (int c = 0; c < CS; ++c) {
-        float acc = st[i].o[c][e] * factor[0];
-#pragma unroll
-        for (int v = 1; v < kWaves; ++v) acc += o_s[((v - 1) * 16 + in_tile) * D + 16 * c + r] * factor[v];
-        partial_o[slot * D + 16 * c + r] = acc;
-      }
+      *reinterpret_cast<floatx4*>(partial_o + slot * D + d) = acc;
     }
   }
 }
 
-// Items: first the shared keys, (tile of rows, split) each; then the sequences' own keys,
-// (sequence, tile of rows, split) each.
-template <typename T, int D, int R>
-__global__ __launch_bounds__(kThreads) void attention_shared_kernel(Batch b, const T* __restrict__ q,
-                                                                    const T* __restrict__ key_pool,
-                                                                    const T* __restrict__ value_pool,
-                                                                    float* __restrict__ partial_o,
-                                                                    float* __restrict__ partial_ml) {
-  __shared__ float lds[2 * kWaves * 16 + (kWaves - 1) * 16 * D];
+constexpr int kColumnWaves = waves_of(128);
+
+// 32 CW rows against the shared keys of ``w`` (at least one): CW waves of 32 columns make a
+// part, and the 8 / CW parts take the pairs in turn, each through LDS buffers of its own.
+template <int D, int CW>
+__device__ __forceinline__ void walk_columns(const Batch& b, const Work& w, const bf16* __restrict__ q,
+                                             const bf16* __restrict__ key_pool, const bf16* __restrict__ value_pool,
+                                             float* __restrict__ partial_o, float* __restrict__ partial_ml,
+                                             void* __restrict__ lds) {
+  constexpr int PARTS = kColumnWaves / CW;
+  constexpr int PART_THREADS = CW * ms::kWave;
+  constexpr int KS = D / 16, CS = ms::PrefillState<D>::CS;
+  using Slot = ms::MergeSlot<D, PARTS>;
+  ms::PairBuffer<D>* buffers = static_cast<ms::PairBuffer<D>*>(lds);       // [parity][part]
+  Slot* slots = static_cast<Slot*>(lds);                                   // [part][wave]
+  const int lane = threadIdx.x & 63;
+  const int wave_of_group = ms::uniform(threadIdx.x >> 6);
+  const int part = wave_of_group / CW, wave = wave_of_group - part * CW;
+  const int thread = threadIdx.x - part * PART_THREADS;
+  const int h = lane >> 5, column = lane & 31;
+  const int per_token = b.num_q_heads / b.num_kv_heads;
+  const int64_t page_stride = static_cast<int64_t>(b.num_kv_heads) * b.block_size * D;
+  const int head_base = w.kv_head * b.block_size * D;
+  const int row = w.row0 + 32 * wave + column;
+  const bool live = row < w.rows;
+  const int token = live ? row / per_token : 0, head = w.kv_head * per_token + (live ? row - token * per_token : 0);
+  const float scale_log2 = b.scale * Operand<bf16>::kScale;
+  const int t0 = w.first_key / kTileKeys, t1 = (w.end_key - 1) / kTileKeys + 1;
+
+  ms::PrefillState<D> st;
+#pragma unroll
+  for (int c = 0; c < CS; ++c)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) st.o[c][v] = 0.f;
+  st.run_max = -INFINITY;
+  st.run_sum = 0.f;
+
+  // Loads are issued kDepth rounds before their pair is consumed (two where a thread stages
+  // little enough), no branch stands around a load, and each buffer is named at compile time.
+  constexpr int kRound = 2 * PARTS;
+  constexpr int kDepth = ms::StagedPair<D, PART_THREADS>::kPerTile > 1 ? 1 : 2;
+  ms::StagedPair<D, PART_THREADS> ahead[kDepth];
+  ms::PairPages pages[kDepth];
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) {
+    const int first = t0 + 2 * part + kRound * i;
+    ms::stage_load<D, PART_THREADS>(ahead[i], thread, ms::find_pair_pages(first, t1, w.table, b.block_size), key_pool,
+                                    value_pool, page_stride, head_base, b.block_size);
+    pages[i] = ms::find_pair_pages(first + kDepth * kRound, t1, w.table, b.block_size);
+  }
+  bf16x8 q_reg[KS];
+#pragma unroll
+  for (int step = 0; step < KS; ++step)
+    q_reg[step] = ms::load_bf16x8(q + (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * D + 16 * step + 8 * h);
+  for (int round_tile = t0; round_tile < t1; round_tile += 2 * kRound) {
+#pragma unroll
+    for (int parity = 0; parity < 2; ++parity) {
+      const int i = kDepth == 2 ? parity : 0;
+      const int t = round_tile + kRound * parity + 2 * part;
+      ms::PairBuffer<D>& buffer = buffers[PARTS * parity + part];
+      ms::stage_store<D, PART_THREADS>(ahead[i], thread, buffer);
+      ms::stage_load<D, PART_THREADS>(ahead[i], thread, pages[i], key_pool, value_pool, page_stride, head_base, b.block_size);
+      pages[i] = ms::find_pair_pages(t + 2 * kDepth * kRound, t1, w.table, b.block_size);
+      __syncthreads();    // the pair is in LDS; every wave is done with the other buffers' previous content
+      if (t < t1)
+        ms::consume_pair<D>(st, buffer, q_reg, t * kTileKeys, w.first_key, w.end_key - 1, w.end_key - 1, scale_log2, h,
+                            column, (t + 2) * kTileKeys > w.end_key);
+    }
+  }
+
+  __syncthreads();    // everybody is done with what the memory held before
+  {
+    Slot& mine = slots[part * CW + wave];
+#pragma unroll
+    for (int c = 0; c < CS; ++c) {
+      if (c % PARTS == part) continue;
+      const int at = 16 * Slot::place(part, c);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mine.value[at + v][lane] = st.o[c][v];
+    }
+    mine.value[16 * Slot::kBlocks][lane] = st.run_max;
+    mine.value[16 * Slot::kBlocks + 1][lane] = st.run_sum;
+  }
+  __syncthreads();
+  if (part >= CS) return;      // no block of outputs is this part's to finish
+  float joint = -INFINITY, total = 0.f, factor[PARTS];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) joint = fmaxf(joint, slots[p * CW + wave].value[16 * Slot::kBlocks][lane]);
+  const float shift = joint == -INFINITY ? 0.f : joint;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const Slot& theirs = slots[p * CW + wave];
+    factor[p] = ms::fast_exp2(theirs.value[16 * Slot::kBlocks][lane] - shift);       // 0 for a part without keys
+    total += theirs.value[16 * Slot::kBlocks + 1][lane] * factor[p];
+  }
+  total += __shfl_xor(total, 32, ms::kWave);      // the column's other lane has the other keys
+  if (!live) return;
+  const int64_t slot = slot_of(b, w, row);
+  if (part == 0 && h == 0) {
+    partial_ml[2 * slot] = joint;
+    partial_ml[2 * slot + 1] = total;
+  }
+#pragma unroll
+  for (int c = 0; c < CS; ++c) {
+    if (c % PARTS != part) continue;
+    float sums[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) sums[v] = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      if (p == part) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[v] = fmaf(st.o[c][v], factor[p], sums[v]);
+      } else {
+        const Slot& theirs = slots[p * CW + wave];
+        const int at = 16 * Slot::place(p, c);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[v] = fmaf(theirs.value[at + v][lane], factor[p], sums[v]);
+      }
+    }
+#pragma unroll
+    for (int quad = 0; quad < 4; ++quad) {
+      const int d = 32 * c + 8 * quad + 4 * h;
+      if (D % 32 != 0 && d >= D) continue;
+      *reinterpret_cast<floatx4*>(partial_o + slot * D + d) =
+          floatx4{sums[4 * quad], sums[4 * quad + 1], sums[4 * quad + 2], sums[4 * quad + 3]};
+    }
+  }
+}
+
+template <typename T, int D, int ROWS>
+constexpr size_t lds_bytes() {
+  constexpr size_t direct = direct_lds_bytes<D, waves_of(ROWS)>();
+  if constexpr (ROWS <= 32) {
+    return direct;
+  } else {
+    constexpr int PARTS = kColumnWaves * 32 / ROWS;
+    constexpr size_t buffers = 2 * PARTS * sizeof(ms::PairBuffer<D>);
+    constexpr size_t slots = kColumnWaves * sizeof(ms::MergeSlot<D, PARTS>);
+    constexpr size_t columns = buffers > slots ? buffers : slots;
+    return columns > direct ? columns : direct;
+  }
+}
+
+// Rows of a tile whose part got no keys.
+__device__ __forceinline__ void leave_empty(const Batch& b, const Work& w, int tile_rows, float* __restrict__ partial_ml) {
+  for (int i = threadIdx.x; i < tile_rows && w.row0 + i < w.rows; i += blockDim.x) {
+    const int64_t slot = slot_of(b, w, w.row0 + i);
+    partial_ml[2 * slot] = -INFINITY;
+    partial_ml[2 * slot + 1] = 0.f;
+  }
+}
+
+// Workgroups: first the shared keys, (kv head, split, tile of ROWS rows) each; then the
+// sequences' own keys, (kv head, split, tile of 16 rows, sequence) each.
+template <typename T, int D, int ROWS>
+__global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) void attention_shared_kernel(
+    Batch b, const T* __restrict__ q, const T* __restrict__ key_pool, const T* __restrict__ value_pool,
+    float* __restrict__ partial_o, float* __restrict__ partial_ml) {
+  constexpr int WAVES = waves_of(ROWS);
+  __shared__ __align__(16) unsigned char lds[lds_bytes<T, D, ROWS>()];
   const int per_token = b.num_q_heads / b.num_kv_heads;
   int item = blockIdx.x;
   Work w;
-  const int shared_items = b.shared_tiles * b.shared_splits;
+  // The tiles of one kv head and split read the same keys: they are handed to one die, where
+  // all but the first find them in the L2 (consecutive workgroups go to the dies in turn).
+  const int units = b.num_kv_heads * b.shared_splits;
+  const int shared_items = (units + kXcds - 1) / kXcds * kXcds * b.shared_tiles;
   if (item < shared_items) {
-    const int tile = item / b.shared_splits, split = item - tile * b.shared_splits;
-    int group, local;
-    if (!find_group_tile(b, tile, per_token, 16 * R, group, local)) return;
+    const int turn = item / kXcds;
+    const int unit = turn / b.shared_tiles * kXcds + item % kXcds;
+    if (unit >= units) return;
+    const int tile = turn % b.shared_tiles, split = unit / b.num_kv_heads;
+    w.kv_head = unit - split * b.num_kv_heads;
+    int group = 0, local = tile, longest = b.shared_lens[0];
+    if (b.num_groups > 1) {
+      longest = longest_shared(b);
+      if (!find_group_tile(b, tile, per_token, ROWS, group, local)) return;
+    }
     const int first_seq = b.group_start[group];
     w.first_token = b.query_start[first_seq];
     w.rows = (b.query_start[b.group_start[group + 1]] - w.first_token) * per_token;
-    w.row0 = local * 16 * R;
+    w.row0 = local * ROWS;
+    if (w.row0 >= w.rows) return;
     const int keys = max(b.shared_lens[group], 0);
-    const int pairs = (keys + 2 * kTileKeys - 1) / (2 * kTileKeys);
-    const int per_split = (pairs + b.shared_splits - 1) / b.shared_splits * 2 * kTileKeys;
-    w.first_key = min(split * per_split, keys);
-    w.end_key = min(w.first_key + per_split, keys);
+    const int per_split = max((longest + b.shared_splits - 1) / b.shared_splits, split_keys(ROWS));
+    const int whole_pairs = (per_split + 2 * kTileKeys - 1) / (2 * kTileKeys) * 2 * kTileKeys;
+    w.first_key = min(split * whole_pairs, keys);
+    w.end_key = min(w.first_key + whole_pairs, keys);
     w.causal = false;
     w.pos_of_first = 0;
     w.table = b.block_table + static_cast<int64_t>(first_seq) * b.max_blocks;
     w.slot = split;
-    walk<T, D, R>(b, w, q, key_pool, value_pool, partial_o, partial_ml, lds);
+    if (w.first_key >= w.end_key) {
+      leave_empty(b, w, ROWS, partial_ml);
+    } else if constexpr (ROWS <= 32) {
+      walk_direct<T, D, ROWS / 16, WAVES>(b, w, q, key_pool, value_pool, partial_o, partial_ml,
+                                          reinterpret_cast<float*>(lds));
+    } else {
+      walk_columns<D, ROWS / 32>(b, w, q, key_pool, value_pool, partial_o, partial_ml, lds);
+    }
     return;
   }
   item -= shared_items;
-  const int seq = item / (b.own_tiles * b.own_splits);
-  item -= seq * b.own_tiles * b.own_splits;
-  const int first_tile = item / b.own_splits, split = item - first_tile * b.own_splits;
-  const int group = group_of_sequence(b, seq);
-  const int context = b.context_lens[seq];
+  w.kv_head = item % b.num_kv_heads;
+  item /= b.num_kv_heads;
+  const int split = item % b.own_splits;
+  item /= b.own_splits;
+  const int first_tile = item % b.own_tiles;
+  const int seq = item / b.own_tiles;
+  const int group = b.num_groups > 1 ? group_of_sequence(b, seq) : seq >= b.group_start[0] && seq < b.group_start[1] ? 0 : -1;
+  const int context = max(b.context_lens[seq], 0);
   w.first_token = b.query_start[seq];
   const int tokens = b.query_start[seq + 1] - w.first_token;
   w.rows = tokens * per_token;
-  w.pos_of_first = context - tokens;
-  const int from = min(group < 0 ? 0 : max(b.shared_lens[group], 0), max(context, 0));
-  // splits begin at a pair of tiles counted from the first own key's tile
+  w.pos_of_first = b.context_lens[seq] - tokens;
+  const int from = min(group < 0 ? 0 : max(b.shared_lens[group], 0), context);
+  // splits begin at whole tiles, counted from the first own key's
   const int start = from / kTileKeys * kTileKeys;
-  const int pairs = (max(context, 0) - start + 2 * kTileKeys - 1) / (2 * kTileKeys);
-  const int per_split = (pairs + b.own_splits - 1) / b.own_splits * 2 * kTileKeys;
-  w.first_key = min(max(start + split * per_split, from), max(context, 0));
-  w.end_key = min(start + (split + 1) * per_split, max(context, 0));
+  const int per_split = max((context - start + b.own_splits - 1) / b.own_splits, split_keys(ROWS));
+  const int whole_pairs = (per_split + 2 * kTileKeys - 1) / (2 * kTileKeys) * 2 * kTileKeys;
+  w.first_key = min(max(start + split * whole_pairs, from), context);
+  w.end_key = min(start + (split + 1) * whole_pairs, context);
   w.causal = true;
   w.table = b.block_table + static_cast<int64_t>(seq) * b.max_blocks;
-  w.slot = b.shared_splits + split;
   for (int tile = first_tile; tile * 16 < w.rows; tile += b.own_tiles) {
-    if (tile != first_tile) __syncthreads();
     w.row0 = tile * 16;
-    walk<T, D, 1>(b, w, q, key_pool, value_pool, partial_o, partial_ml, lds);
+    w.slot = b.shared_splits + split;
+    if (w.first_key >= w.end_key) {
+      leave_empty(b, w, 16, partial_ml);
+    } else {
+      if (tile != first_tile) __syncthreads();      // what the tile before left in LDS is read
+      walk_direct<T, D, 1, WAVES>(b, w, q, key_pool, value_pool, partial_o, partial_ml, reinterpret_cast<float*>(lds));
+    }
     if (group < 0 && split == 0) {
       // no workgroup makes shared parts for a sequence without a group: they are empty
-      for (int i = threadIdx.x; i < 16 * b.shared_splits; i += kThreads) {
-        const int row = w.row0 + i / b.shared_splits;
-        if (row >= w.rows) break;
-        const int64_t slot = (static_cast<int64_t>(w.first_token + row / per_token) * b.num_q_heads +
-                              blockIdx.y * per_token + row % per_token) * (b.shared_splits + b.own_splits) +
-                             i % b.shared_splits;
-        partial_ml[2 * slot] = -INFINITY;
-        partial_ml[2 * slot + 1] = 0.f;
-      }
+      for (w.slot = 0; w.slot < b.shared_splits; ++w.slot) leave_empty(b, w, 16, partial_ml);
     }
   }
 }
 
 // Joins the parts of a row, a wave each.  A row that saw no key gives zeros, and so do the
 // rows of tokens behind the last sequence.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(const float* __restrict__ partial_o,
-                                                                         const float* __restrict__ partial_ml,
-                                                                         const int32_t* __restrict__ query_start,
-                                                                         T* __restrict__ out, int64_t rows,
-                                                                         int num_seqs, int num_q_heads, int head_dim,
-                                                                         int slots) {
+constexpr int kJoinWaves = 4;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kJoinWaves * ms::kWave) void attention_shared_join_kernel(const float* __restrict__ partial_o,
+                                                                                 const float* __restrict__ partial_ml,
+                                                                                 const int32_t* __restrict__ query_start,
+                                                                                 T* __restrict__ out, int64_t rows,
+                                                                                 int num_seqs, int num_q_heads, int slots) {
+  constexpr int kLanes = D / 4;                       // a part's output, four values a lane
+  constexpr int kAtOnce = ms::kWave / kLanes;         // parts that the wave reads with one instruction
+  constexpr int kDeep = 8;                            // of those instructions in flight
   const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinWaves + (threadIdx.x >> 6);
   if (row >= rows) return;
+  const int group = min(lane / kLanes, kAtOnce), d = 4 * (lane % kLanes);
+  const bool reads = group < kAtOnce;
+  const float* from = partial_o + row * slots * D + d;
+  // the first parts are on their way while the weights are made; what an empty part holds is not used
+  floatx4 ahead[kDeep];
+#pragma unroll
+  for (int u = 0; u < kDeep; ++u)
+    ahead[u] = *reinterpret_cast<const floatx4*>(from + static_cast<int64_t>(min(group + u * kAtOnce, slots - 1)) * D);
   const bool live = row / num_q_heads < query_start[num_seqs];
-  float m[2], l[2], mx = -INFINITY;
+  float m[2], mx = -INFINITY, l[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int s = lane + 64 * h;
@@ -460,42 +720,72 @@ __global__ __launch_bounds__(kThreads) void attention_shared_join_kernel(const f
   }
   total = ms::wave_sum(total);
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  for (int d = lane; d < head_dim; d += ms::kWave) {
-    float acc = 0.f;
-    if (live) {
-#pragma unroll 4
-      for (int s = 0; s < slots; ++s) {
-        const float factor = __shfl(s < 64 ? m[0] : m[1], s & 63, ms::kWave);
-        const float value = partial_o[(row * slots + s) * head_dim + d];
-        acc = factor > 0.f ? fmaf(factor, value, acc) : acc;      // the output of an empty part was never written
-      }
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < slots; first += kDeep * kAtOnce) {
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int s = first + group + u * kAtOnce;
+      const float near = __shfl(m[0], s & 63, ms::kWave), far = __shfl(m[1], s & 63, ms::kWave);
+      const float factor = s >= slots || !reads ? 0.f : s < 64 ? near : far;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = factor > 0.f ? fmaf(factor, ahead[u][e], acc[e]) : acc[e];
     }
-    out[row * head_dim + d] = ms::from_float<T>(acc * inv);
+    if (first + kDeep * kAtOnce < slots) {
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u)
+        ahead[u] = *reinterpret_cast<const floatx4*>(
+            from + static_cast<int64_t>(min(first + (kDeep + u) * kAtOnce + group, slots - 1)) * D);
+    }
   }
+  // the lanes' shares of a value, added up in the order of the groups
+  floatx4 sum = acc;
+#pragma unroll
+  for (int other = 1; other < kAtOnce; ++other)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl(acc[e], (lane + other * kLanes) & 63, ms::kWave);
+  if (lane >= kLanes) return;
+  T* to = out + row * D + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = ms::from_float<T>(sum[e] * inv);
 }
 
 template <typename T, int D>
-void launch(const Batch& b, int rows_per_tile, const void* q, const void* key_pool, const void* value_pool,
-            void* partial_o, void* partial_ml, hipStream_t stream) {
-  const int64_t items = static_cast<int64_t>(b.shared_tiles) * b.shared_splits +
-                        static_cast<int64_t>(b.num_seqs) * b.own_tiles * b.own_splits;
-  const dim3 grid(static_cast<unsigned>(items), b.num_kv_heads);
-#define MS_SHARED_ROWS(R)                                                                                          \
-  hipLaunchKernelGGL((attention_shared_kernel<T, D, R>), grid, dim3(kThreads), 0, stream, b, static_cast<const T*>(q), \
-                     static_cast<const T*>(key_pool), static_cast<const T*>(value_pool),                           \
-                     static_cast<float*>(partial_o), static_cast<float*>(partial_ml))
-  if (rows_per_tile == 16) MS_SHARED_ROWS(1);
-  else MS_SHARED_ROWS(2);
+int launch(const Batch& b, const void* q, const void* key_pool, const void* value_pool, void* out, void* partial_o,
+           void* partial_ml, hipStream_t stream) {
+  const int units = b.num_kv_heads * b.shared_splits;
+  const int64_t items = static_cast<int64_t>((units + kXcds - 1) / kXcds * kXcds) * b.shared_tiles +
+                        static_cast<int64_t>(b.num_seqs) * b.own_tiles * b.own_splits * b.num_kv_heads;
+  MS_REQUIRE(items < (1LL << 31) / (8 * ms::kWave), "attention_shared_prefix: the batch is too large");
+#define MS_SHARED_ROWS(ROWS)                                                                                       \
+  hipLaunchKernelGGL((attention_shared_kernel<T, D, ROWS>), dim3(static_cast<unsigned>(items)),                 \
+                     dim3(waves_of(ROWS) * ms::kWave), 0, \
+                     stream, b, static_cast<const T*>(q), static_cast<const T*>(key_pool),                         \
+                     static_cast<const T*>(value_pool), static_cast<float*>(partial_o), static_cast<float*>(partial_ml))
+  if constexpr (sizeof(T) == 2) {
+    if (b.tile_rows == 128) MS_SHARED_ROWS(128);
+    else if (b.tile_rows == 64) MS_SHARED_ROWS(64);
+    else if (b.tile_rows == 32) MS_SHARED_ROWS(32);
+    else MS_SHARED_ROWS(16);
+  } else {
+    MS_SHARED_ROWS(16);
+  }
 #undef MS_SHARED_ROWS
+  MS_CHECK_LAUNCH("attention_shared_prefix");
+  const int64_t rows = static_cast<int64_t>(b.num_tokens) * b.num_q_heads;
+  hipLaunchKernelGGL((attention_shared_join_kernel<T, D>), dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)),
+                     dim3(kJoinWaves * ms::kWave), 0, stream, static_cast<const float*>(partial_o),
+                     static_cast<const float*>(partial_ml), b.query_start, static_cast<T*>(out), rows, b.num_seqs,
+                     b.num_q_heads, b.shared_splits + b.own_splits);
+  MS_CHECK_LAUNCH("attention_shared_prefix (join)");
+  return 0;
 }
 
 template <typename T>
-int run_shared(const Batch& b, int head_dim, int rows_per_tile, const void* q, const void* key_pool,
-               const void* value_pool, void* out, void* partial_o, void* partial_ml, hipStream_t stream) {
-#define MS_SHARED_CASE(DIM)                                                                        \
-  case DIM:                                                                                        \
-    launch<T, DIM>(b, rows_per_tile, q, key_pool, value_pool, partial_o, partial_ml, stream);      \
-    break;
+int run_shared(const Batch& b, int head_dim, const void* q, const void* key_pool, const void* value_pool, void* out,
+               void* partial_o, void* partial_ml, hipStream_t stream) {
+#define MS_SHARED_CASE(DIM) \
+  case DIM:                 \
+    return launch<T, DIM>(b, q, key_pool, value_pool, out, partial_o, partial_ml, stream);
   switch (head_dim) {
     MS_SHARED_CASE(16) MS_SHARED_CASE(32) MS_SHARED_CASE(48) MS_SHARED_CASE(64) MS_SHARED_CASE(80)
     MS_SHARED_CASE(96) MS_SHARED_CASE(112) MS_SHARED_CASE(128)
@@ -503,14 +793,6 @@ int run_shared(const Batch& b, int head_dim, int rows_per_tile, const void* q, c
       return ms_fail("attention_shared_prefix: head_dim %d", head_dim);
   }
 #undef MS_SHARED_CASE
-  MS_CHECK_LAUNCH("attention_shared_prefix");
-  const int64_t rows = static_cast<int64_t>(b.num_tokens) * b.num_q_heads;
-  hipLaunchKernelGGL((attention_shared_join_kernel<T>), dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)),
-                     dim3(kThreads), 0, stream, static_cast<const float*>(partial_o),
-                     static_cast<const float*>(partial_ml), b.query_start, static_cast<T*>(out), rows, b.num_seqs,
-                     b.num_q_heads, head_dim, b.shared_splits + b.own_splits);
-  MS_CHECK_LAUNCH("attention_shared_prefix (join)");
-  return 0;
 }
 
 }  // namespace
@@ -524,8 +806,8 @@ extern "C" int ms_attention_shared_prefix_supported(int head_dim, int block_size
 // q, out: [num_tokens, num_q_heads, head_dim]; pools as for ms_attention_decode; query_start
 // [num_seqs + 1], context_lens [num_seqs], group_start [num_groups + 1], shared_lens
 // [num_groups]; partial_o: float [num_tokens, num_q_heads, shared_splits + own_splits,
-// head_dim]; partial_ml: the same with 2 in head_dim's place.  rows_per_tile: 16 or 32 rows
-// of a group a workgroup; own_tiles: workgroups that share a sequence's tiles of 16 rows.
+// head_dim]; partial_ml: the same with 2 in head_dim's place.  rows_per_tile: 16, 32, 64
+// or 128 rows of a group a workgroup (32-bit storage: 16); own_tiles: workgroups that share a sequence's tiles of 16 rows.
 extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, const void* value_pool,
                                           const void* block_table, const void* query_start, const void* context_lens,
                                           const void* group_start, const void* shared_lens, void* out, void* partial_o,
@@ -535,18 +817,21 @@ extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, c
                                           int own_tiles, int own_splits, int dtype, hipStream_t stream) {
   MS_REQUIRE(num_tokens > 0 && num_seqs > 0 && num_groups > 0 && max_blocks > 0,
              "attention_shared_prefix: nothing to do (%d tokens, %d sequences, %d groups)", num_tokens, num_seqs, num_groups);
-  MS_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_kv_heads <= 65535 && num_q_heads % num_kv_heads == 0,
+  MS_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0,
              "attention_shared_prefix: %d query heads are not a multiple of %d kv heads", num_q_heads, num_kv_heads);
   MS_REQUIRE(ms_attention_shared_prefix_supported(head_dim, block_size),
              "attention_shared_prefix: head_dim %d (multiples of 16 up to 128) or block_size %d (multiples of 16) is not supported",
              head_dim, block_size);
-  MS_REQUIRE(rows_per_tile == 16 || rows_per_tile == 32, "attention_shared_prefix: tiles of %d rows", rows_per_tile);
+  MS_REQUIRE(rows_per_tile == 16 || (dtype == MS_BF16 && (rows_per_tile == 32 || rows_per_tile == 64 || rows_per_tile == 128)),
+             "attention_shared_prefix: tiles of %d rows", rows_per_tile);
+  MS_REQUIRE(static_cast<int64_t>(num_kv_heads) * block_size * head_dim < (int64_t{1} << 31),
+             "attention_shared_prefix: a page of %d kv heads x %d keys x %d is too large", num_kv_heads, block_size, head_dim);
   MS_REQUIRE(shared_splits >= 1 && shared_splits <= kMaxSplits && own_splits >= 1 && own_splits <= kMaxSplits && own_tiles >= 1,
              "attention_shared_prefix: %d and %d splits are outside 1..%d", shared_splits, own_splits, kMaxSplits);
   MS_REQUIRE(dtype == MS_F32 || dtype == MS_BF16, "attention_shared_prefix: unknown dtype %d", dtype);
   const int64_t rows = static_cast<int64_t>(num_tokens) * (num_q_heads / num_kv_heads);
   MS_REQUIRE(rows < (1LL << 31) - 4096 && rows / rows_per_tile + num_groups < (1LL << 24) / shared_splits &&
-                 static_cast<int64_t>(num_seqs) * own_tiles * own_splits < (1LL << 24),
+                 static_cast<int64_t>(num_seqs) * own_tiles * own_splits < (1LL << 31) / num_kv_heads,
              "attention_shared_prefix: the batch is too large");
   Batch b;
   b.block_table = static_cast<const int32_t*>(block_table);
@@ -563,11 +848,13 @@ extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, c
   b.max_blocks = max_blocks;
   b.scale = scale;
   // every group has at most one tile that is not full
-  b.shared_tiles = static_cast<int>(rows / rows_per_tile) + num_groups;
+  b.tile_rows = rows_per_tile;
+  b.shared_tiles = num_groups == 1 ? static_cast<int>((rows + rows_per_tile - 1) / rows_per_tile)
+                                   : static_cast<int>(rows / rows_per_tile) + num_groups;
   b.shared_splits = shared_splits;
   b.own_tiles = own_tiles;
   b.own_splits = own_splits;
   if (dtype == MS_F32)
-    return run_shared<float>(b, head_dim, rows_per_tile, q, key_pool, value_pool, out, partial_o, partial_ml, stream);
-  return run_shared<bf16>(b, head_dim, rows_per_tile, q, key_pool, value_pool, out, partial_o, partial_ml, stream);
+    return run_shared<float>(b, head_dim, q, key_pool, value_pool, out, partial_o, partial_ml, stream);
+  return run_shared<bf16>(b, head_dim, q, key_pool, value_pool, out, partial_o, partial_ml, stream);
 }

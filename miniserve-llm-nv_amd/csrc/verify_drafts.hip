@@ -24,12 +24,32 @@
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / ms::kWave;
-constexpr int kQuads = 4;                               // quads of elements a thread holds
-constexpr int kChunk = kThreads * kQuads * 4;           // elements of a chunk
+// Elements of a row that a wave takes in (1), 32 to a lane (the waves of a workgroup share
+// nothing, so none waits for another), and that a workgroup takes in (2) and (3), where the row
+// is one of the request's and many units share it.
+constexpr int kRowChunk = 2048, kChunk = 4096;
+constexpr int kRowThreads = 256, kChooseThreads = 512, kDrawThreads = kChunk / 4;
+
+// 2^f on -1/2 .. 1/2, lowest power first: the polynomial of degree nine whose largest relative
+// error there is least (found by exchange of its extrema: 1.3e-14).  It travels with a kernel's
+// arguments, so that its coefficients lie in scalar registers: as literals the compiler copies
+// each into vector registers before every use (39 instructions an element instead of 25).
+constexpr int kDegree = 9;
+constexpr double kPowerOfTwo[kDegree + 1] = {
+    1.00000000000001266e+00,
+    6.93147180559871012e-01,
+    2.40226506956496527e-01,
+    5.55041086686855825e-02,
+    9.61812919206720199e-03,
+    1.33335576176098788e-03,
+    1.54034349480814238e-04,
+    1.52529848355783673e-05,
+    1.32594056112041923e-06,
+    1.01503372609764174e-07,
+};
 
 struct Batch {
+  double power[kDegree + 1];
   const float* __restrict__ logits;
   const int32_t* __restrict__ row_start;
   const int32_t* __restrict__ draft_tokens;
@@ -37,7 +57,7 @@ struct Batch {
   const float* __restrict__ accept_uniform;
   const float* __restrict__ draw_uniform;
   const float* __restrict__ temperature;        // or null: all 0
-  int rows, vocab, requests, chunks;
+  int rows, vocab, requests, row_chunks, chunks;
 };
 
 struct RowPart {
@@ -78,91 +98,90 @@ __device__ __forceinline__ float temperature_of(const Batch& b, int request) {
   return b.temperature != nullptr ? b.temperature[request] : 0.f;
 }
 
-// The thread's elements of a chunk, four quads that lie on 16-byte borders of the row's
-// memory: element(j, i) of quad j, values outside the row left at `outside`.
-struct Quads {
-  float value[kQuads][4];
-  int first[kQuads];
-};
-
-__device__ __forceinline__ void load_quads(Quads& q, const float* __restrict__ row, int vocab, int chunk, int shift,
-                                           float outside) {
-  const bool aligned = ((reinterpret_cast<uintptr_t>(row) >> 2) & 3) == static_cast<uintptr_t>(shift);
+// 2^x in 64 bits for x <= 0: 2^k 2^f with k the nearest whole number.  (1) is bound by these
+// instructions, so that k is had by adding 3 * 2^51, which leaves it in the sum's low bits, and
+// 2^k by adding k to the exponent's bits (conversions and scalings run at a quarter of an
+// addition's rate).  Below 2^-1000 the result is 2^-1000 at most and not 0.
+__device__ __forceinline__ double pow2_floored(const Batch& b, double x) {
+  x = fmax(x, -1001.0);
+  const double shifted = x + 6755399441055744.0;
+  const double f = x - (shifted - 6755399441055744.0);
+  double r = b.power[kDegree];
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j) {
-    q.first[j] = chunk * kChunk + 4 * (threadIdx.x + j * kThreads) - shift;
-    const int e = q.first[j];
-    if (aligned && e >= 0 && e + 3 < vocab) {
-      const float4 four = *reinterpret_cast<const float4*>(row + e);
-      q.value[j][0] = four.x, q.value[j][1] = four.y, q.value[j][2] = four.z, q.value[j][3] = four.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q.value[j][i] = e + i >= 0 && e + i < vocab ? row[e + i] : outside;
-    }
-  }
+  for (int n = kDegree - 1; n >= 0; --n) r = fma(r, f, b.power[n]);
+  return __hiloint2double(__double2hiint(r) + (__double2loint(shifted) << 20), __double2loint(r));
 }
+__device__ __forceinline__ double pow2(const Batch& b, double x) { return x < -1000.0 ? 0.0 : pow2_floored(b, x); }
+
+// e^{(l - max) / temperature} = 2^{(l - max) * rate}
+__device__ __forceinline__ double rate_of(float temperature) { return 1.4426950408889634074 / static_cast<double>(temperature); }
+__device__ __forceinline__ double exponent_of(float logit, float max, double rate) {
+  return (static_cast<double>(logit) - static_cast<double>(max)) * rate;
+}
+__device__ __forceinline__ double mass_of(const Batch& b, float logit, float max, double rate) {
+  return pow2(b, exponent_of(logit, max, rate));
+}
+
+__device__ __forceinline__ bool not_finite(float v) { return __builtin_isfpclass(v, 0x3 | 0x4 | 0x200); }      // NaN, -inf, +inf
 
 __device__ __forceinline__ int shift_of(const float* row) { return static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 2) & 3); }
 
-__device__ __forceinline__ double wave_sum_double(double v) {
+typedef float Four __attribute__((ext_vector_type(4)));
+
+// A thread's elements of a chunk: quads that lie on 16-byte borders of the row's memory;
+// quad j is value[j], its first element first[j].
+template <int QUADS>
+struct Quads {
+  float value[QUADS][4];
+  int first[QUADS];
+  bool whole;       // no element of the chunk lies outside the row (the same in all threads)
+};
+
+// ``shift``: floats between the 16-byte border before the row and the row.  What lies outside
+// the row is left at `outside`.
+template <int QUADS, int THREADS>
+__device__ __forceinline__ void load_quads(Quads<QUADS>& q, int thread, const float* __restrict__ row, int vocab, int begin,
+                                           int shift, float outside) {
+  // no branch around the loads of a chunk that lies inside the row: all are under way at once
+  q.whole = shift_of(row) == shift && begin >= shift && begin - shift + 4 * QUADS * THREADS <= vocab;
 #pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, ms::kWave);
+  for (int j = 0; j < QUADS; ++j) q.first[j] = begin + 4 * (thread + j * THREADS) - shift;
+  if (q.whole) {
+#pragma unroll
+    for (int j = 0; j < QUADS; ++j) {
+      const Four four = *reinterpret_cast<const Four*>(row + q.first[j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.value[j][i] = four[i];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < QUADS; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = q.first[j] + i;
+        const float v = row[min(max(e, 0), vocab - 1)];
+        q.value[j][i] = e >= 0 && e < vocab ? v : outside;
+      }
+  }
+}
+
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
+#pragma unroll
+  for (int offset = LANES / 2; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, LANES);
   return v;
 }
 
-__device__ __forceinline__ double block_sum_double(double v, double* scratch) {
-  v = wave_sum_double(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double total = 0.0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += scratch[w];
-  return total;
-}
-
-// (1) grid (chunks, rows)
-__global__ __launch_bounds__(kThreads) void verify_rows_kernel(Batch b, RowPart* __restrict__ parts) {
-  __shared__ float max_s[kWaves];
-  __shared__ int place_s[kWaves];
-  __shared__ double sum_s[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int chunk = blockIdx.x, row = blockIdx.y;
+// (1) grid (chunks of a row, four to a workgroup; rows)
+__global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(Batch b, RowPart* __restrict__ parts) {
+  constexpr int kQuads = kRowChunk / ms::kWave / 4;
+  const int lane = threadIdx.x & 63;
+  const int chunk = blockIdx.x * (kRowThreads / ms::kWave) + ms::uniform(threadIdx.x >> 6), row = blockIdx.y;
+  if (chunk >= b.row_chunks) return;
   const float* logits = b.logits + static_cast<int64_t>(row) * b.vocab;
-  const float outside = -3.402823466e38f;
-  Quads q;
-  load_quads(q, logits, b.vocab, chunk, shift_of(logits), outside);
-  float best = -INFINITY;
-  int place = 0x7fffffff;
-  bool bad = false;
-#pragma unroll
-  for (int j = 0; j < kQuads; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = q.first[j] + i;
-      const float v = q.value[j][i];
-      if (!(fabsf(v) <= 3.402823466e38f)) bad = true;
-      if (e >= 0 && e < b.vocab && (v > best || (v == best && e < place))) best = v, place = e;
-    }
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) {
-    const float other = __shfl_xor(best, offset, ms::kWave);
-    const int other_place = __shfl_xor(place, offset, ms::kWave);
-    if (other > best || (other == best && other_place < place)) best = other, place = other_place;
-  }
-  bad = __any(bad);
-  if (lane == 0) {
-    max_s[wave] = best;
-    place_s[wave] = bad ? -1 : place;
-  }
-  __syncthreads();
-  best = max_s[0], place = place_s[0];
-  bad = place < 0;
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    bad = bad || place_s[w] < 0;
-    if (max_s[w] > best || (max_s[w] == best && place_s[w] < place)) best = max_s[w], place = place_s[w];
-  }
+  constexpr float kOutside = -3.402823466e38f;          // finite, and no more than any finite number of the row
+  Quads<kQuads> q;
+  load_quads<kQuads, ms::kWave>(q, lane, logits, b.vocab, chunk * kRowChunk, shift_of(logits), kOutside);
   // the request of the row, for its temperature
   float temperature = 0.f;
   if (b.temperature != nullptr) {
@@ -173,24 +192,51 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Batch b, RowPart*
     }
     temperature = b.temperature[max(at_or_before - 1, 0)];
   }
+  float best = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bad |= not_finite(q.value[j][i]);
+      best = fmaxf(best, q.value[j][i]);
+    }
+  best = ms::wave_max(best);
+  bad = __any(bad);
   double sum = 0.0;
-  if (temperature > 0.f && !bad) {
-    const double factor = 1.0 / static_cast<double>(temperature);
+  int place = 0x7fffffff;
+  if (temperature > 0.f) {
+    const double rate = rate_of(temperature);
+    // (a sum that holds a mass of 1 does not see one of 2^-1000)
+    if (q.whole) {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += pow2_floored(b, exponent_of(q.value[j][i], best, rate));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = q.first[j] + i;
+          const double mass = pow2_floored(b, exponent_of(q.value[j][i], best, rate));
+          sum += e >= 0 && e < b.vocab ? mass : 0.0;
+        }
+    }
+    sum = lanes_sum<ms::kWave>(sum);
+  } else {
+    // the lowest index of the maximum
 #pragma unroll
     for (int j = 0; j < kQuads; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = q.first[j] + i;
-        if (e >= 0 && e < b.vocab) sum += exp((static_cast<double>(q.value[j][i]) - static_cast<double>(best)) * factor);
+        if (q.value[j][i] == best && e >= 0 && e < b.vocab) place = min(place, e);
       }
-    sum = block_sum_double(sum, sum_s);
+#pragma unroll
+    for (int offset = 32; offset > 0; offset >>= 1) place = min(place, __shfl_xor(place, offset, ms::kWave));
   }
-  if (threadIdx.x == 0) {
-    RowPart& part = parts[static_cast<int64_t>(row) * b.chunks + chunk];
-    part.sum = sum;
-    part.max = best;
-    part.place = bad ? -1 : place;
-  }
+  if (lane == 0) parts[static_cast<int64_t>(row) * b.row_chunks + chunk] = RowPart{sum, best, bad ? -1 : place};
 }
 
 struct RowSums {
@@ -199,91 +245,141 @@ struct RowSums {
   int place;      // -1: not finite
 };
 
-// A row's maximum, its place and its sum from the chunks'; by one wave, the same in all lanes.
-__device__ __forceinline__ RowSums row_sums(const Batch& b, const RowPart* __restrict__ parts, int row, double factor) {
-  const int lane = threadIdx.x & 63;
+// A row's maximum, its place and its sum from the chunks'; by 32 lanes, the same in all of them.
+__device__ __forceinline__ RowSums row_sums(const Batch& b, const RowPart* __restrict__ parts, int row, double rate) {
+  const int lane = threadIdx.x & 31;
   RowSums r{0.0, -INFINITY, 0x7fffffff};
+  constexpr int kHeld = 3;        // chunks a lane keeps: 196,608 tokens of the vocabulary
+  RowPart held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int c = lane + 32 * u;
+    held[u] = c < b.row_chunks ? parts[static_cast<int64_t>(row) * b.row_chunks + c] : RowPart{0.0, -INFINITY, 0x7fffffff};
+  }
   bool bad = false;
-  for (int c = lane; c < b.chunks; c += ms::kWave) {
-    const RowPart part = parts[static_cast<int64_t>(row) * b.chunks + c];
+  const auto look = [&](const RowPart& part) {
     bad = bad || part.place < 0;
     if (part.max > r.max || (part.max == r.max && part.place < r.place)) r.max = part.max, r.place = part.place;
-  }
+  };
 #pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) {
-    const float other = __shfl_xor(r.max, offset, ms::kWave);
-    const int other_place = __shfl_xor(r.place, offset, ms::kWave);
+  for (int u = 0; u < kHeld; ++u) look(held[u]);
+  for (int c = lane + 32 * kHeld; c < b.row_chunks; c += 32) look(parts[static_cast<int64_t>(row) * b.row_chunks + c]);
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) {
+    const float other = __shfl_xor(r.max, offset, 32);
+    const int other_place = __shfl_xor(r.place, offset, 32);
+    bad |= __shfl_xor(static_cast<int>(bad), offset, 32) != 0;
     if (other > r.max || (other == r.max && other_place < r.place)) r.max = other, r.place = other_place;
   }
-  if (__any(bad)) r.place = -1;
-  if (factor > 0.0 && r.place >= 0) {
-    double sum = 0.0;
-    for (int c = lane; c < b.chunks; c += ms::kWave) {
-      const RowPart part = parts[static_cast<int64_t>(row) * b.chunks + c];
-      sum += part.sum * exp((static_cast<double>(part.max) - static_cast<double>(r.max)) * factor);
-    }
-    r.sum = wave_sum_double(sum);
-  }
+  if (bad) r.place = -1;
+  double sum = 0.0;
+  const auto add = [&](const RowPart& part) {
+    if (part.sum > 0.0) sum += part.sum * mass_of(b, part.max, r.max, rate);
+  };
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) add(held[u]);
+  for (int c = lane + 32 * kHeld; c < b.row_chunks; c += 32) add(parts[static_cast<int64_t>(row) * b.row_chunks + c]);
+  r.sum = lanes_sum<32>(sum);
   return r;
 }
 
-// (2) grid (chunks, requests)
-__global__ __launch_bounds__(kThreads) void verify_choose_kernel(Batch b, const RowPart* __restrict__ parts,
-                                                                 Masses* __restrict__ masses,
-                                                                 Decision* __restrict__ decisions) {
-  __shared__ int end_s[kWaves];
-  __shared__ double sum_s[kWaves];
-  const int lane = threadIdx.x & 63, wave = ms::uniform(threadIdx.x >> 6);
-  const int chunk = blockIdx.x, request = blockIdx.y;
-  const Rows rows = rows_of(b, request);
-  const float temperature = temperature_of(b, request);
+// How a request ends; by a whole workgroup, the same in all its threads.
+__device__ __forceinline__ Decision decide(const Batch& b, const RowPart* __restrict__ parts, int request, const Rows& rows,
+                                           float temperature) {
+  constexpr int kWaves = kChooseThreads / ms::kWave;
+  constexpr int kAtOnce = kChooseThreads / 32;       // rows that are looked at together, 32 lanes each
+  __shared__ RowSums sums_s[kAtOnce];
+  __shared__ uint64_t ends_s[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = threadIdx.x >> 5;
   const bool greedy = !(temperature > 0.f);
-  const double factor = greedy ? 0.0 : 1.0 / static_cast<double>(temperature);
-  // each wave looks at drafts of its own; the first that is not taken ends them
-  int end = rows.drafts;
-  for (int i = wave; i < rows.drafts && i < end; i += kWaves) {
-    const int row = rows.first + i;
-    const int64_t draft = rows.first_draft + i;
-    const RowSums sums = row_sums(b, parts, row, factor);
-    const int token = b.draft_tokens[draft];
-    bool taken = false;
-    if (sums.place >= 0 && token >= 0 && token < b.vocab) {
-      if (greedy) {
-        taken = token == sums.place;
-      } else {
-        const double logit = b.logits[static_cast<int64_t>(row) * b.vocab + token];
-        const double p = exp((logit - static_cast<double>(sums.max)) * factor) / sums.sum;
-        const double q = b.draft_probs != nullptr ? b.draft_probs[draft * b.vocab + token] : 1.f;
-        taken = static_cast<double>(b.accept_uniform[draft]) * q < p;
+  const double rate = greedy ? 0.0 : rate_of(temperature);
+  // the first row whose draft is not taken; the row behind the last draft has none
+  int end = 0;
+  for (int first = 0;; first += kAtOnce) {
+    const int i = first + half;
+    bool ends = i == rows.drafts;
+    if (i <= rows.drafts) {
+      const int row = rows.first + i;
+      const int64_t draft = rows.first_draft + i;
+      double mass = 0.0, q = 1.0, u = 0.0;
+      int token = -1;
+      if (!ends) {
+        token = b.draft_tokens[draft];
+        if (!greedy && token >= 0 && token < b.vocab) {
+          u = b.accept_uniform[draft];
+          mass = b.logits[static_cast<int64_t>(row) * b.vocab + token];
+          if (b.draft_probs != nullptr) q = b.draft_probs[draft * b.vocab + token];
+        }
       }
+      const RowSums sums = row_sums(b, parts, row, rate);
+      if (!ends) {
+        if (sums.place < 0 || token < 0 || token >= b.vocab) {
+          ends = true;
+        } else if (greedy) {
+          ends = token != sums.place;
+        } else {
+          ends = !(u * q < mass_of(b, static_cast<float>(mass), sums.max, rate) / sums.sum);
+        }
+      }
+      if ((threadIdx.x & 31) == 0) sums_s[half] = sums;
     }
-    if (!taken) end = i;
-  }
-  if (lane == 0) end_s[wave] = end;
-  __syncthreads();
+    const uint64_t found = __ballot(ends);      // lane 0: the wave's first row, lane 32: its second
+    if (lane == 0) ends_s[wave] = found;
+    __syncthreads();
+    int at = -1;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) end = min(end, end_s[w]);
-  const int row = rows.first + end;
-  const RowSums sums = row_sums(b, parts, row, factor);
-  const bool chosen = greedy || sums.place < 0;
-  const int64_t draft = end < rows.drafts ? rows.first_draft + end : -1;
-  if (chunk == 0 && threadIdx.x == 0) {
-    Decision& d = decisions[request];
-    d.inverse_sum = chosen ? 0.0 : 1.0 / sums.sum;
-    d.max = sums.max;
-    d.row = row;
-    d.accepted = end;
-    d.token = chosen ? sums.place : -2;
-    d.draft = static_cast<int32_t>(draft);
+    for (int w = kWaves - 1; w >= 0; --w) {
+      if (ends_s[w] >> 32 & 1) at = 2 * w + 1;
+      if (ends_s[w] & 1) at = 2 * w;
+    }
+    if (at >= 0) {
+      end = first + at;
+      break;
+    }
+    __syncthreads();
   }
-  if (chosen) return;
-  const double inverse = 1.0 / sums.sum;
-  const float* logits = b.logits + static_cast<int64_t>(row) * b.vocab;
+  const RowSums sums = sums_s[end % kAtOnce];
+  const bool chosen = greedy || sums.place < 0;
+  return Decision{1.0 / sums.sum, sums.max, rows.first + end, end, chosen ? sums.place : -2,
+                  end < rows.drafts ? rows.first_draft + end : -1};
+}
+
+// (2a) grid (requests), for many requests: the decisions by themselves.  A workgroup of (2)
+// takes some 5 us to make its request's, in which its unit draws nothing from memory; with
+// few requests that is shorter than another kernel.
+__global__ __launch_bounds__(kChooseThreads) void verify_decide_kernel(Batch b, const RowPart* __restrict__ parts,
+                                                                       Decision* __restrict__ decisions) {
+  const int request = blockIdx.x;
+  const Decision d = decide(b, parts, request, rows_of(b, request), temperature_of(b, request));
+  if (threadIdx.x == 0) decisions[request] = d;
+}
+
+// (2) grid (chunks, requests)
+template <bool DECIDED>
+__global__ __launch_bounds__(kChooseThreads) void verify_choose_kernel(Batch b, const RowPart* __restrict__ parts,
+                                                                       Masses* __restrict__ masses,
+                                                                       Decision* __restrict__ decisions) {
+  constexpr int kWaves = kChooseThreads / ms::kWave, kQuads = kChunk / kChooseThreads / 4;
+  __shared__ double residual_s[kWaves], plain_s[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int chunk = blockIdx.x, request = blockIdx.y;
+  const float temperature = temperature_of(b, request);
+  Decision d;
+  if constexpr (DECIDED) {
+    d = decisions[request];
+  } else {
+    d = decide(b, parts, request, rows_of(b, request), temperature);
+    if (chunk == 0 && threadIdx.x == 0) decisions[request] = d;
+  }
+  if (d.token != -2) return;
+  const double rate = rate_of(temperature), inverse = d.inverse_sum;
+  const int64_t draft = d.draft;
+  const float* logits = b.logits + static_cast<int64_t>(d.row) * b.vocab;
   const int shift = shift_of(logits);
-  Quads l, q;
-  load_quads(l, logits, b.vocab, chunk, shift, 0.f);
+  Quads<kQuads> l, q;
+  load_quads<kQuads, kChooseThreads>(l, threadIdx.x, logits, b.vocab, chunk * kChunk, shift, 0.f);
   const bool subtract = draft >= 0 && b.draft_probs != nullptr;
-  if (subtract) load_quads(q, b.draft_probs + draft * b.vocab, b.vocab, chunk, shift, 0.f);
+  if (subtract) load_quads<kQuads, kChooseThreads>(q, threadIdx.x, b.draft_probs + draft * b.vocab, b.vocab, chunk * kChunk, shift, 0.f);
   const int without = draft >= 0 && b.draft_probs == nullptr ? b.draft_tokens[draft] : -1;
   double residual = 0.0, plain = 0.0;
 #pragma unroll
@@ -292,91 +388,110 @@ __global__ __launch_bounds__(kThreads) void verify_choose_kernel(Batch b, const 
     for (int i = 0; i < 4; ++i) {
       const int e = l.first[j] + i;
       if (e < 0 || e >= b.vocab) continue;
-      const double p = exp((static_cast<double>(l.value[j][i]) - static_cast<double>(sums.max)) * factor) * inverse;
+      const double p = mass_of(b, l.value[j][i], d.max, rate) * inverse;
       plain += p;
       residual += subtract ? fmax(p - static_cast<double>(q.value[j][i]), 0.0) : (e == without ? 0.0 : p);
     }
-  residual = block_sum_double(residual, sum_s);
-  plain = block_sum_double(plain, sum_s);
-  if (threadIdx.x == 0) masses[static_cast<int64_t>(request) * b.chunks + chunk] = Masses{residual, plain};
+  residual = lanes_sum<ms::kWave>(residual);
+  plain = lanes_sum<ms::kWave>(plain);
+  if (lane == 0) residual_s[wave] = residual, plain_s[wave] = plain;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Masses m{0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m.residual += residual_s[w], m.plain += plain_s[w];
+    masses[static_cast<int64_t>(request) * b.chunks + chunk] = m;
+  }
+}
+
+// Running sums over the lanes of a wave, this lane's included.
+__device__ __forceinline__ double wave_running_sum(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int offset = 1; offset < ms::kWave; offset <<= 1) {
+    const double other = __shfl_up(v, offset, ms::kWave);
+    if (lane >= offset) v += other;
+  }
+  return v;
 }
 
 // (3) grid (requests)
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(Batch b, const Masses* __restrict__ masses,
-                                                               const Decision* __restrict__ decisions,
-                                                               int32_t* __restrict__ tokens,
-                                                               int32_t* __restrict__ accepted) {
+__global__ __launch_bounds__(kDrawThreads) void verify_draw_kernel(Batch b, const Masses* __restrict__ masses,
+                                                                   const Decision* __restrict__ decisions,
+                                                                   int32_t* __restrict__ tokens,
+                                                                   int32_t* __restrict__ accepted) {
+  constexpr int kWaves = kDrawThreads / ms::kWave;
   __shared__ double wave_s[kWaves];
-  __shared__ int chunk_s, token_s;
-  __shared__ double before_s, target_s;
-  __shared__ bool residual_s;
+  __shared__ int passed_s[kWaves], last_s[kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int request = blockIdx.x;
   const Rows rows = rows_of(b, request);
   const Decision d = decisions[request];
   int token = d.token;
   if (token == -2) {
-    if (threadIdx.x == 0) {
-      const Masses* m = masses + static_cast<int64_t>(request) * b.chunks;
-      double residual = 0.0, plain = 0.0;
-      for (int c = 0; c < b.chunks; ++c) residual += m[c].residual, plain += m[c].plain;
-      const bool use = residual > 0.0;
-      const double target = static_cast<double>(b.draw_uniform[request]) * (use ? residual : plain);
-      double before = 0.0, running = 0.0;
-      int chunk = 0;
-      for (int c = 0; c < b.chunks; ++c) {
-        const double mass = use ? m[c].residual : m[c].plain;
-        if (mass > 0.0) {
-          chunk = c;
-          before = running;
-          running += mass;
-          if (running > target) break;
-        }
+    // the chunk in which the running sum passes the target; by every wave for itself
+    const Masses* m = masses + static_cast<int64_t>(request) * b.chunks;
+    const double uniform = b.draw_uniform[request];
+    const Masses mine = lane < b.chunks ? m[lane] : Masses{0.0, 0.0};
+    double residual = mine.residual, plain = mine.plain;
+    for (int c = lane + ms::kWave; c < b.chunks; c += ms::kWave) residual += m[c].residual, plain += m[c].plain;
+    residual = lanes_sum<ms::kWave>(residual);
+    plain = lanes_sum<ms::kWave>(plain);
+    const bool use = residual > 0.0;
+    const double target = uniform * (use ? residual : plain);
+    double carried = 0.0, before = 0.0;
+    int chunk = 0;
+    for (int c0 = 0; c0 < b.chunks; c0 += ms::kWave) {
+      const int c = c0 + lane;
+      const Masses here = c0 == 0 ? mine : c < b.chunks ? m[c] : Masses{0.0, 0.0};
+      const double mass = use ? here.residual : here.plain;
+      const double upto = wave_running_sum(mass);
+      const uint64_t some = __ballot(mass > 0.0), past = __ballot(mass > 0.0 && carried + upto > target);
+      if (some != 0) {
+        // where rounding leaves no chunk that passes, the last one with a mass
+        const int at = past != 0 ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+        chunk = c0 + at;
+        before = carried + __shfl(upto - mass, at, ms::kWave);
+        if (past != 0) break;
       }
-      chunk_s = chunk, before_s = before, target_s = target, residual_s = use;
-      token_s = -1;
+      carried += __shfl(upto, ms::kWave - 1, ms::kWave);
     }
-    __syncthreads();
-    // the chunk's elements in their order, kQuads * 4 neighbours a thread
+    // the chunk's elements in their order, four neighbours a thread
     const float* logits = b.logits + static_cast<int64_t>(d.row) * b.vocab;
-    const double factor = 1.0 / static_cast<double>(temperature_of(b, request));
-    const bool subtract = residual_s && d.draft >= 0 && b.draft_probs != nullptr;
-    const int without = residual_s && d.draft >= 0 && b.draft_probs == nullptr ? b.draft_tokens[d.draft] : -1;
-    const float* probs = subtract ? b.draft_probs + static_cast<int64_t>(d.draft) * b.vocab : nullptr;
-    const int first = chunk_s * kChunk - shift_of(logits) + threadIdx.x * kQuads * 4;
-    double mass[kQuads * 4], sum = 0.0;
+    const int shift = shift_of(logits);
+    const double rate = rate_of(temperature_of(b, request));
+    const bool subtract = use && d.draft >= 0 && b.draft_probs != nullptr;
+    const int without = use && d.draft >= 0 && b.draft_probs == nullptr ? b.draft_tokens[d.draft] : -1;
+    Quads<1> l, q;
+    load_quads<1, kDrawThreads>(l, threadIdx.x, logits, b.vocab, chunk * kChunk, shift, 0.f);
+    if (subtract) load_quads<1, kDrawThreads>(q, threadIdx.x, b.draft_probs + static_cast<int64_t>(d.draft) * b.vocab, b.vocab, chunk * kChunk, shift, 0.f);
+    double mass[4], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kQuads * 4; ++i) {
-      const int e = first + i;
+    for (int i = 0; i < 4; ++i) {
+      const int e = l.first[0] + i;
       mass[i] = 0.0;
       if (e >= 0 && e < b.vocab && e != without) {
-        const double p = exp((static_cast<double>(logits[e]) - static_cast<double>(d.max)) * factor) * d.inverse_sum;
-        mass[i] = subtract ? fmax(p - static_cast<double>(probs[e]), 0.0) : p;
+        const double p = mass_of(b, l.value[0][i], d.max, rate) * d.inverse_sum;
+        mass[i] = subtract ? fmax(p - static_cast<double>(q.value[0][i]), 0.0) : p;
       }
       sum += mass[i];
     }
-    double upto = sum;
-#pragma unroll
-    for (int offset = 1; offset < ms::kWave; offset <<= 1) {
-      const double other = __shfl_up(upto, offset, ms::kWave);
-      if (lane >= offset) upto += other;
-    }
+    const double upto = wave_running_sum(sum);
     if (lane == ms::kWave - 1) wave_s[wave] = upto;
     __syncthreads();
-    double running = before_s + upto - sum;
+    double running = before + upto - sum;
     for (int w = 0; w < wave; ++w) running += wave_s[w];
     // the first element at which the running sum passes the target; where rounding leaves
     // none (the target lies at the chunk's very end), the last one with a mass
     int passed = 0x7fffffff, last = -1;
 #pragma unroll
-    for (int i = 0; i < kQuads * 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
       running += mass[i];
       if (mass[i] > 0.0) {
-        last = first + i;
-        if (running > target_s && passed == 0x7fffffff) passed = first + i;
+        last = l.first[0] + i;
+        if (running > target && passed == 0x7fffffff) passed = l.first[0] + i;
       }
     }
-    __shared__ int passed_s[kWaves], last_s[kWaves];
 #pragma unroll
     for (int offset = 32; offset > 0; offset >>= 1) {
       passed = min(passed, __shfl_xor(passed, offset, ms::kWave));
@@ -384,18 +499,21 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Batch b, const Ma
     }
     if (lane == 0) passed_s[wave] = passed, last_s[wave] = last;
     __syncthreads();
+    if (wave == 0) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) passed = min(passed, passed_s[w]), last = max(last, last_s[w]);
-    token = passed != 0x7fffffff ? passed : last;
+      for (int w = 1; w < kWaves; ++w) passed = min(passed, passed_s[w]), last = max(last, last_s[w]);
+      token = passed != 0x7fffffff ? passed : last;
+    }
   }
-  for (int i = threadIdx.x; i <= rows.drafts; i += kThreads) {
+  if (wave != 0) return;
+  for (int i = lane; i <= rows.drafts; i += ms::kWave) {
     const int row = rows.first + i;
     tokens[row] = i < d.accepted ? b.draft_tokens[rows.first_draft + i] : i == d.accepted ? token : -1;
   }
-  if (threadIdx.x == 0) accepted[request] = d.accepted;
+  if (lane == 0) accepted[request] = d.accepted;
 }
 
-int chunks_of(int vocab) { return (vocab + 3 + kChunk - 1) / kChunk; }      // a row may begin at any float of a quad
+int chunks_of(int vocab, int chunk) { return (vocab + 3 + chunk - 1) / chunk; }      // a row may begin at any float of a quad
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -405,9 +523,8 @@ size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // the vocabulary.
 extern "C" size_t ms_verify_drafts_workspace_bytes(int rows, int requests, int vocab) {
   if (rows <= 0 || requests <= 0 || vocab <= 0) return 0;
-  const size_t chunks = chunks_of(vocab);
-  return aligned(rows * chunks * sizeof(RowPart)) + aligned(requests * chunks * sizeof(Masses)) +
-         aligned(requests * sizeof(Decision));
+  return aligned(sizeof(RowPart) * rows * chunks_of(vocab, kRowChunk)) +
+         aligned(sizeof(Masses) * requests * chunks_of(vocab, kChunk)) + aligned(sizeof(Decision) * requests);
 }
 
 // logits: float [rows, vocab]; row_start: int32 [requests + 1], request r's rows are
@@ -426,6 +543,7 @@ extern "C" int ms_verify_drafts(const void* logits, const void* row_start, const
   MS_REQUIRE(draft_tokens != nullptr || rows == requests, "verify_drafts: no drafted tokens");
   MS_REQUIRE(workspace_bytes >= ms_verify_drafts_workspace_bytes(rows, requests, vocab), "verify_drafts: workspace too small");
   Batch b;
+  for (int n = 0; n <= kDegree; ++n) b.power[n] = kPowerOfTwo[n];
   b.logits = static_cast<const float*>(logits);
   b.row_start = static_cast<const int32_t*>(row_start);
   b.draft_tokens = static_cast<const int32_t*>(draft_tokens);
@@ -436,19 +554,31 @@ extern "C" int ms_verify_drafts(const void* logits, const void* row_start, const
   b.rows = rows;
   b.vocab = vocab;
   b.requests = requests;
-  b.chunks = chunks_of(vocab);
+  b.row_chunks = chunks_of(vocab, kRowChunk);
+  b.chunks = chunks_of(vocab, kChunk);
   char* at = static_cast<char*>(workspace);
   RowPart* parts = reinterpret_cast<RowPart*>(at);
-  at += aligned(static_cast<size_t>(rows) * b.chunks * sizeof(RowPart));
+  at += aligned(sizeof(RowPart) * rows * b.row_chunks);
   Masses* masses = reinterpret_cast<Masses*>(at);
-  at += aligned(static_cast<size_t>(requests) * b.chunks * sizeof(Masses));
+  at += aligned(sizeof(Masses) * requests * b.chunks);
   Decision* decisions = reinterpret_cast<Decision*>(at);
-  hipLaunchKernelGGL(verify_rows_kernel, dim3(b.chunks, rows), dim3(kThreads), 0, stream, b, parts);
+  hipLaunchKernelGGL(verify_rows_kernel, dim3((b.row_chunks + kRowThreads / ms::kWave - 1) / (kRowThreads / ms::kWave), rows),
+                     dim3(kRowThreads), 0, stream, b, parts);
   MS_CHECK_LAUNCH("verify_drafts (rows)");
-  hipLaunchKernelGGL(verify_choose_kernel, dim3(b.chunks, requests), dim3(kThreads), 0, stream, b,
-                     static_cast<const RowPart*>(parts), masses, decisions);
+  const dim3 grid(b.chunks, requests);
+  // decisions apart where the workgroups of (2) do not all run at once
+  if (static_cast<int64_t>(b.chunks) * requests > 2 * ms_compute_units()) {
+    hipLaunchKernelGGL(verify_decide_kernel, dim3(requests), dim3(kChooseThreads), 0, stream, b,
+                       static_cast<const RowPart*>(parts), decisions);
+    MS_CHECK_LAUNCH("verify_drafts (decide)");
+    hipLaunchKernelGGL((verify_choose_kernel<true>), grid, dim3(kChooseThreads), 0, stream, b,
+                       static_cast<const RowPart*>(parts), masses, decisions);
+  } else {
+    hipLaunchKernelGGL((verify_choose_kernel<false>), grid, dim3(kChooseThreads), 0, stream, b,
+                       static_cast<const RowPart*>(parts), masses, decisions);
+  }
   MS_CHECK_LAUNCH("verify_drafts (choose)");
-  hipLaunchKernelGGL(verify_draw_kernel, dim3(requests), dim3(kThreads), 0, stream, b, static_cast<const Masses*>(masses),
+  hipLaunchKernelGGL(verify_draw_kernel, dim3(requests), dim3(kDrawThreads), 0, stream, b, static_cast<const Masses*>(masses),
                      static_cast<const Decision*>(decisions), static_cast<int32_t*>(tokens),
                      static_cast<int32_t*>(accepted));
   MS_CHECK_LAUNCH("verify_drafts (draw)");

@@ -83,14 +83,19 @@ def _check(tensor: torch.Tensor, name: str, *, dtype: torch.dtype | None = None,
         raise KernelError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}.")
 
 
-def _check_on_current_device(**tensors: torch.Tensor | None) -> None:
-    """All on the GPU that is current: kernels are launched there, on its current stream."""
+def _address(tensor: torch.Tensor | None, name: str, device: int, dtype: torch.dtype, shape: tuple | None = None) -> int | None:
+    """The address of a tensor after the checks of :func:`_check`, and that it lives on the
+    GPU that is current (``device``), on whose stream kernels are launched; None for None.
+    (One pass over what a right tensor answers: a serving step makes some hundred calls.)"""
 
-    current = torch.cuda.current_device()
-    for name, tensor in tensors.items():
-        if tensor is not None and tensor.device.index != current:
-            raise KernelError(f"{name} lives on {tensor.device}, the current device is cuda:{current}; "
-                              "make the tensors' device current (torch.cuda.device).")
+    if tensor is None:
+        return None
+    if not (isinstance(tensor, torch.Tensor) and tensor.get_device() == device and tensor.dtype is dtype
+            and tensor.is_contiguous() and (shape is None or tensor.shape == shape)):
+        _check(tensor, name, dtype=dtype, shape=shape)
+        raise KernelError(f"{name} lives on {tensor.device}, the current device is cuda:{device}; "
+                          "make the tensors' device current (torch.cuda.device).")
+    return tensor.data_ptr()
 
 
 def _ptr(tensor: torch.Tensor | None) -> int | None:
@@ -432,19 +437,28 @@ def can_share_prefix(head_dim: int, block_size: int) -> bool:
 
 
 def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, per_token: int, max_shared: int,
-                         max_own: int, max_query: int) -> tuple[int, int, int, int]:
+                         max_own: int, max_query: int, dtype: torch.dtype) -> tuple[int, int, int, int]:
     """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
     the parts those keys are cut into, the workgroups that share a sequence's tiles of 16
     rows, and the parts that its own keys are cut into.  ``rows``: tokens times query heads
     of a kv head."""
 
-    target = _decode_target()
-    tile = 16 if rows <= 16 * groups else 32
+    units = _decode_target() // 2
+    tile = 16
+    while dtype == torch.bfloat16 and tile < 128 and tile * groups < rows:
+        tile *= 2
     tiles = max(groups, -(-rows // tile))
-    shared_splits = max(1, min(-(-target // (tiles * kv_heads)), -(-max_shared // 128), _DECODE_MAX_SPLITS))
+    # a compute unit holds two workgroups of four waves (tiles of few rows) or one of eight;
+    # a wave has a pair of 16-key tiles at least
+    waves, room = (4, 2 * units) if tile <= 32 else (8, units)
+
+    def splits(parts: int, most: int, keys: int) -> int:
+        return max(1, min(most // parts, -(-keys // (32 * waves)), _DECODE_MAX_SPLITS))
+
     own_tiles = -(-max_query * per_token // 16)
-    own_splits = max(1, min(-(-target // (sequences * own_tiles * kv_heads)), max_own // 160, _DECODE_MAX_SPLITS))
-    return tile, shared_splits, own_tiles, own_splits
+    # groups of different lengths have their keys cut into parts of the same length: more of them, to fill the gaps
+    return (tile, splits(tiles * kv_heads, room if groups == 1 else 2 * room, max_shared), own_tiles,
+            splits(sequences * own_tiles * kv_heads, room, max_own))
 
 
 def attention_shared_prefix(
@@ -489,28 +503,29 @@ def attention_shared_prefix(
     if q.ndim != 3 or q.numel() == 0:
         raise KernelError("attention_shared_prefix: q must be [N>0, heads>0, head_dim>0].")
     n, heads, head_dim = q.shape
-    _check(key_pool, "key_pool", dtype=q.dtype)
+    dtype, device = q.dtype, torch.cuda.current_device()
+    code = _code(dtype)
+    q_at = _address(q, "q", device, dtype)
+    keys_at = _address(key_pool, "key_pool", device, dtype)
     if key_pool.ndim != 4 or key_pool.shape[3] != head_dim or key_pool.numel() == 0:
         raise KernelError(
             f"attention_shared_prefix: pool {tuple(key_pool.shape)} is not [pages, kv_heads, block_size, {head_dim}]."
         )
-    _check(value_pool, "value_pool", dtype=q.dtype, shape=_value_pool_shape(key_pool))
-    _, kv_heads, block_size, _ = key_pool.shape
+    pages, kv_heads, block_size, _ = key_pool.shape
+    values_at = _address(value_pool, "value_pool", device, dtype, (pages, kv_heads, head_dim, block_size))
     if heads % kv_heads != 0:
         raise KernelError(f"attention_shared_prefix: {heads} query heads are not a multiple of {kv_heads} kv heads.")
-    _check(block_table, "block_table", dtype=torch.int32)
+    table_at = _address(block_table, "block_table", device, torch.int32)
     if block_table.ndim != 2 or block_table.numel() == 0:
         raise KernelError("attention_shared_prefix: block_table must be [S>0, max_blocks>0].")
     sequences, max_blocks = block_table.shape
-    _check(query_start, "query_start", dtype=torch.int32, shape=(sequences + 1,))
-    _check(context_lens, "context_lens", dtype=torch.int32, shape=(sequences,))
-    _check(group_start, "group_start", dtype=torch.int32)
+    starts_at = _address(query_start, "query_start", device, torch.int32, (sequences + 1,))
+    contexts_at = _address(context_lens, "context_lens", device, torch.int32, (sequences,))
+    groups_at = _address(group_start, "group_start", device, torch.int32)
     if group_start.ndim != 1 or group_start.numel() < 2:
         raise KernelError("attention_shared_prefix: group_start must be [groups + 1] for at least one group.")
     groups = group_start.numel() - 1
-    _check(shared_lens, "shared_lens", dtype=torch.int32, shape=(groups,))
-    _check_on_current_device(q=q, key_pool=key_pool, value_pool=value_pool, block_table=block_table, query_start=query_start,
-                             context_lens=context_lens, group_start=group_start, shared_lens=shared_lens)
+    shared_at = _address(shared_lens, "shared_lens", device, torch.int32, (groups,))
     longest = max_blocks * block_size
     bounds = []
     for name, given, most in (("max_shared", max_shared, longest), ("max_own", max_own, longest), ("max_query", max_query, n)):
@@ -518,15 +533,15 @@ def attention_shared_prefix(
             raise KernelError(f"attention_shared_prefix: {name} must be a whole number or None, not {given!r}.")
         bounds.append(max(1, most if given is None else min(given, most)))
     per_token = heads // kv_heads
-    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, groups, sequences, kv_heads, per_token, *bounds)
+    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, groups, sequences, kv_heads, per_token, *bounds, dtype)
     out = torch.empty_like(q)
-    slots = shared_splits + own_splits
-    partial_o = torch.empty((n, heads, slots, head_dim), dtype=torch.float32, device=q.device)
-    partial_ml = torch.empty((n, heads, slots, 2), dtype=torch.float32, device=q.device)
-    call("ms_attention_shared_prefix", _ptr(q), _ptr(key_pool), _ptr(value_pool), _ptr(block_table), _ptr(query_start),
-         _ptr(context_lens), _ptr(group_start), _ptr(shared_lens), _ptr(out), _ptr(partial_o), _ptr(partial_ml), n, sequences,
-         groups, heads, kv_heads, head_dim, block_size, max_blocks, float(scale), tile, shared_splits, own_tiles, own_splits,
-         _code(q.dtype), _stream())
+    # of every part of a row's keys the outputs, then the maximum and the sum
+    parts = n * heads * (shared_splits + own_splits)
+    workspace = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
+    partial_o = workspace.data_ptr()
+    call("ms_attention_shared_prefix", q_at, keys_at, values_at, table_at, starts_at, contexts_at, groups_at, shared_at,
+         out.data_ptr(), partial_o, partial_o + 4 * parts * head_dim, n, sequences, groups, heads, kv_heads, head_dim, block_size,
+         max_blocks, float(scale), tile, shared_splits, own_tiles, own_splits, code, _stream())
     attention_calls["shared"] += 1
     return out
 
@@ -542,20 +557,21 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
 
     if not isinstance(pools, (list, tuple)) or not pools:
         raise KernelError("copy_pages takes a list of at least one pool.")
+    described = []
     for index, pool in enumerate(pools):
         _check(pool, f"pools[{index}]")
         if pool.ndim < 3 or pool.numel() == 0:
             raise KernelError(f"copy_pages: pools[{index}] {tuple(pool.shape)} is not [calls>0, pages>0, ...].")
-    _check_on_current_device(**{f"pools[{index}]": pool for index, pool in enumerate(pools)})
+        at = _address(pool, f"pools[{index}]", torch.cuda.current_device(), pool.dtype)
+        described.append((at, pool.stride(1) * pool.element_size(), pool.shape[0], pool.shape[1]))
     count = len(source)
     if len(destination) != count:
         raise KernelError(f"copy_pages: {count} pages to {len(destination)} places.")
     if count == 0:
         return
-    for page in (*source, *destination):
-        if type(page) is not int:
-            raise KernelError(f"copy_pages: a page is named by a whole number, not {page!r}.")
-    fewest = min(pool.shape[1] for pool in pools)
+    if {*map(type, source), *map(type, destination)} != {int}:
+        raise KernelError("copy_pages: pages are named by whole numbers.")
+    fewest = min(pages for *_, pages in described)
     if min(source) < 0 or max(source) >= fewest or min(destination) < 0 or max(destination) >= fewest:
         raise KernelError(f"copy_pages: a page lies outside the pools' {fewest}.")
     places = set(destination)
@@ -563,15 +579,14 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
         raise KernelError("copy_pages: a page is the destination of two copies.")
     if not places.isdisjoint(source):
         raise KernelError("copy_pages: a page is the source of one copy and the destination of another.")
-    from_pages, to_pages = (ctypes.c_int32 * count)(*source), (ctypes.c_int32 * count)(*destination)
+    numbers = (ctypes.c_int32 * count)
+    from_pages, to_pages = numbers(*source), numbers(*destination)
     most = int(load().ms_copy_pages_most_pools())
-    for first in range(0, len(pools), most):
-        some = pools[first : first + most]
-        bases = (ctypes.c_void_p * len(some))(*(pool.data_ptr() for pool in some))
-        page_bytes = (ctypes.c_int64 * len(some))(*(pool[0, 0].numel() * pool.element_size() for pool in some))
-        calls = (ctypes.c_int32 * len(some))(*(pool.shape[0] for pool in some))
-        pages = (ctypes.c_int32 * len(some))(*(pool.shape[1] for pool in some))
-        call("ms_copy_pages", bases, page_bytes, calls, pages, len(some), from_pages, to_pages, count, _stream())
+    for first in range(0, len(described), most):
+        some = described[first : first + most]
+        bases, page_bytes, calls, pages = zip(*some)
+        call("ms_copy_pages", (ctypes.c_void_p * len(some))(*bases), (ctypes.c_int64 * len(some))(*page_bytes),
+             (ctypes.c_int32 * len(some))(*calls), (ctypes.c_int32 * len(some))(*pages), len(some), from_pages, to_pages, count, _stream())
 
 
 _EPILOGUE_BF16, _EPILOGUE_F32, _EPILOGUE_ADD_F32, _EPILOGUE_SILU_MUL = 0, 1, 2, 3
@@ -1085,27 +1100,27 @@ def verify_drafts(
     if logits.ndim != 2 or logits.numel() == 0:
         raise KernelError("verify_drafts takes logits [R>0, V>0].")
     rows, vocab = logits.shape
-    _check(row_start, "row_start", dtype=torch.int32)
+    device = torch.cuda.current_device()
+    logits_at = _address(logits, "logits", device, torch.float32)
+    starts_at = _address(row_start, "row_start", device, torch.int32)
     if row_start.ndim != 1 or not 2 <= row_start.numel() <= rows + 1:
         raise KernelError(f"verify_drafts: row_start must be [requests + 1] for 1 to {rows} requests.")
     requests = row_start.numel() - 1
-    _check(draft_tokens, "draft_tokens", dtype=torch.int32, shape=(rows - requests,))
-    if draft_probs is not None:
-        _check(draft_probs, "draft_probs", dtype=torch.float32, shape=(rows - requests, vocab))
+    drafts = (rows - requests,)
+    tokens_at = _address(draft_tokens, "draft_tokens", device, torch.int32, drafts)
+    probs_at = _address(draft_probs, "draft_probs", device, torch.float32, (rows - requests, vocab))
+    accept_at = draw_at = heat_at = None
     if temperature is not None:
-        _check(temperature, "temperature", dtype=torch.float32, shape=(requests,))
         if accept_uniform is None or draw_uniform is None:
             raise KernelError("verify_drafts: sampling needs uniform numbers.")
-        _check(accept_uniform, "accept_uniform", dtype=torch.float32, shape=(rows - requests,))
-        _check(draw_uniform, "draw_uniform", dtype=torch.float32, shape=(requests,))
-    _check_on_current_device(logits=logits, row_start=row_start, draft_tokens=draft_tokens, draft_probs=draft_probs,
-                             accept_uniform=accept_uniform, draw_uniform=draw_uniform, temperature=temperature)
-    tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    accepted = torch.empty((requests,), dtype=torch.int32, device=logits.device)
+        heat_at = _address(temperature, "temperature", device, torch.float32, (requests,))
+        accept_at = _address(accept_uniform, "accept_uniform", device, torch.float32, drafts)
+        draw_at = _address(draw_uniform, "draw_uniform", device, torch.float32, (requests,))
+    out = torch.empty(rows + requests, dtype=torch.int32, device=logits.device)
+    tokens, accepted = out.split((rows, requests))
     size = int(load().ms_verify_drafts_workspace_bytes(rows, requests, vocab))
     workspace = torch.empty(size, dtype=torch.uint8, device=logits.device)
-    # without drafts their tensors are empty, and their addresses null
-    call("ms_verify_drafts", _ptr(logits), _ptr(row_start), _ptr(draft_tokens), _ptr(draft_probs) if rows > requests else None,
-         _ptr(accept_uniform), _ptr(draw_uniform), _ptr(temperature), _ptr(tokens), _ptr(accepted), _ptr(workspace), size,
-         rows, requests, vocab, _stream())
+    out_at = out.data_ptr()
+    call("ms_verify_drafts", logits_at, starts_at, tokens_at, probs_at if rows > requests else None, accept_at, draw_at, heat_at,
+         out_at, out_at + 4 * rows, workspace.data_ptr(), size, rows, requests, vocab, _stream())
     return tokens, accepted

@@ -376,9 +376,10 @@ def test_the_cut_of_the_work_stays_within_what_the_kernel_takes(monkeypatch):
         groups = rng.randint(1, sequences)
         kv_heads, per_token, query = rng.choice([1, 2, 8]), rng.choice([1, 2, 3, 8, 24]), rng.choice([1, 2, 9, 70])
         longest = rng.choice([1, 100, 5000, 10**6])
-        launch = ops.shared_prefix_launch(sequences * query * per_token, groups, sequences, kv_heads, per_token, longest, longest, query)
+        dtype = rng.choice([torch.float32, torch.bfloat16])
+        launch = ops.shared_prefix_launch(sequences * query * per_token, groups, sequences, kv_heads, per_token, longest, longest, query, dtype)
         tile, shared_splits, own_tiles, own_splits = launch
-        assert tile in (16, 32) and 1 <= shared_splits <= 64 and 1 <= own_splits <= 64 and own_tiles >= 1
+        assert tile in ((16, 32, 64, 128) if dtype == torch.bfloat16 else (16,)) and 1 <= shared_splits <= 64 and 1 <= own_splits <= 64 and own_tiles >= 1
 
 
 def test_the_plain_check_of_drafted_tokens_by_hand():

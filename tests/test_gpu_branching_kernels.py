@@ -130,6 +130,16 @@ def test_many_groups_of_all_sizes(ops, dtype):
     check_attention(ops, attention_case(dtype, 8, 2, 32, 16, groups, seed=3))
 
 
+@pytest.mark.parametrize("rows", [16, 17, 33, 64, 65, 100, 128, 129, 200, 300])
+@pytest.mark.parametrize("dim,page", [(64, 16), (80, 48), (128, 16), (112, 32), (32, 64)])
+def test_rows_of_a_group_around_every_tile(ops, rows, dim, page):
+    # one kv head, as many query heads: rows = sequences times heads
+    heads = next(h for h in (4, 3, 5, 1) if rows % h == 0)
+    members = [(1, 1 + i % 5) for i in range(rows // heads)]
+    for shared in (page, 13 * page + 1, 700):
+        check_attention(ops, attention_case(torch.bfloat16, heads, 1, dim, page, [(shared, members)], seed=rows + shared))
+
+
 def test_more_groups_than_a_wave_has_lanes(ops):
     groups = [(16 * (1 + g % 3), [(1, 1 + g % 7)] * (1 + g % 2)) for g in range(131)]
     check_attention(ops, attention_case(torch.bfloat16, 4, 2, 32, 16, groups, seed=4))
@@ -519,7 +529,7 @@ def test_refusals_of_the_gpu_side(ops):
         ("list of at least one", pool, [0], [1]), ("outside", [pool], [5], [1]), ("outside", [pool], [-1], [1]), ("outside", [pool], [1], [5]),
         ("outside", [pool, torch.zeros(2, 3, 8, device=DEVICE)], [4], [1]), ("two copies", [pool], [0, 1], [2, 2]),
         ("source of one copy", [pool], [0, 1], [1, 2]), ("source of one copy", [pool], [3], [3]), ("1 pages to 2", [pool], [0], [1, 2]),
-        ("whole number", [pool], [0.0], [1]), ("whole number", [pool], [True], [2]), ("contiguous", [pool[:, :, ::2]], [0], [1]),
+        ("whole numbers", [pool], [0.0], [1]), ("whole numbers", [pool], [True], [2]), ("contiguous", [pool[:, :, ::2]], [0], [1]),
         ("calls>0", [torch.zeros(5, device=DEVICE)], [0], [1]),
     ]:
         with pytest.raises(KernelError, match=match):
