@@ -23,6 +23,22 @@
 //            to serve as many of them as possible).
 //
 // The waves' (m, l, O) are joined through LDS, so a workgroup leaves one part a row.
+//
+// Measured on MI355X (bf16, head size 128, 8 kv heads, both kernels, recorded in a graph):
+//
+//   2 rows of 16 heads over 512 shared keys       8 us   start of two kernels and the chain
+//                                                        table -> keys -> products of each
+//   8 rows of 32 heads over 2,048                11 us   the same
+//   45 rows of 32 heads, 7 groups of up to       39 us   161 MB in 33 us at a copy's rate; the
+//     5,000 and up to 700 keys of their own               sequences' own keys are most of it
+//   64 rows of 64 heads over 30,000              96 us   63 GFLOP: 0.66 PFLOP/s.  The products alone
+//                                                        take 52 us at a large product's rate, the
+//                                                        exponentials and conversions between them
+//                                                        as much again, and the waves of a unit
+//                                                        overlap only some of it
+//
+// With every sequence reading its keys for itself the last three take 89 us (45 rows), 138 us
+// (16 rows with 5 tokens each over 4,096, here 19) and 632 us.
 #include "attention_columns.hpp"
 
 namespace {
@@ -104,15 +120,22 @@ struct Operand<float> {
 
 // ---- where work lies ----------------------------------------------------------------
 
-struct Batch {
-  const int32_t* __restrict__ block_table;
-  const int32_t* __restrict__ query_start;
-  const int32_t* __restrict__ context_lens;
-  const int32_t* __restrict__ group_start;
-  const int32_t* __restrict__ shared_lens;
+struct Sizes {
   int num_tokens, num_seqs, num_groups, num_q_heads, num_kv_heads, block_size, max_blocks;
   float scale;
   int tile_rows, shared_tiles, shared_splits, own_tiles, own_splits;
+};
+
+// What a kernel is called with, as its functions see it.  (The pointers are arguments of their
+// own, and not part of a struct that is passed: only so does the compiler know that no store
+// changes the tables, and reads them with scalar loads.  A vector load of a page number waits
+// for all loads of keys that are under way.)
+struct Batch : Sizes {
+  const int32_t* block_table;
+  const int32_t* query_start;
+  const int32_t* context_lens;
+  const int32_t* group_start;
+  const int32_t* shared_lens;
 };
 
 // Rows and keys of one workgroup, the same in all its lanes.
@@ -462,7 +485,9 @@ __device__ __forceinline__ void walk_columns(const Batch& b, const Work& w, cons
   const bool live = row < w.rows;
   const int token = live ? row / per_token : 0, head = w.kv_head * per_token + (live ? row - token * per_token : 0);
   const float scale_log2 = b.scale * Operand<bf16>::kScale;
-  const int t0 = w.first_key / kTileKeys, t1 = (w.end_key - 1) / kTileKeys + 1;
+  // Whole pairs of tiles in the loop, which need no masks; a rest of fewer than 32 keys behind it.
+  const int t0 = w.first_key / kTileKeys, t1 = t0 + (w.end_key - w.first_key) / (2 * kTileKeys) * 2;
+  const int end_tile = (w.end_key - 1) / kTileKeys + 1;
 
   ms::PrefillState<D> st;
 #pragma unroll
@@ -472,6 +497,12 @@ __device__ __forceinline__ void walk_columns(const Batch& b, const Work& w, cons
   st.run_max = -INFINITY;
   st.run_sum = 0.f;
 
+  // The queries are asked for before the first keys: loads come back in their order, and a wait
+  // for later ones, which the compiler repeats in every round, would be one for the keys ahead.
+  bf16x8 q_reg[KS];
+#pragma unroll
+  for (int step = 0; step < KS; ++step)
+    q_reg[step] = ms::load_bf16x8(q + (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * D + 16 * step + 8 * h);
   // Loads are issued kDepth rounds before their pair is consumed (two where a thread stages
   // little enough), no branch stands around a load, and each buffer is named at compile time.
   constexpr int kRound = 2 * PARTS;
@@ -481,14 +512,10 @@ __device__ __forceinline__ void walk_columns(const Batch& b, const Work& w, cons
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) {
     const int first = t0 + 2 * part + kRound * i;
-    ms::stage_load<D, PART_THREADS>(ahead[i], thread, ms::find_pair_pages(first, t1, w.table, b.block_size), key_pool,
+    ms::stage_load<D, PART_THREADS>(ahead[i], thread, ms::find_pair_pages(first, end_tile, w.table, b.block_size), key_pool,
                                     value_pool, page_stride, head_base, b.block_size);
-    pages[i] = ms::find_pair_pages(first + kDepth * kRound, t1, w.table, b.block_size);
+    pages[i] = ms::find_pair_pages(first + kDepth * kRound, end_tile, w.table, b.block_size);
   }
-  bf16x8 q_reg[KS];
-#pragma unroll
-  for (int step = 0; step < KS; ++step)
-    q_reg[step] = ms::load_bf16x8(q + (static_cast<int64_t>(w.first_token + token) * b.num_q_heads + head) * D + 16 * step + 8 * h);
   for (int round_tile = t0; round_tile < t1; round_tile += 2 * kRound) {
 #pragma unroll
     for (int parity = 0; parity < 2; ++parity) {
@@ -497,12 +524,24 @@ __device__ __forceinline__ void walk_columns(const Batch& b, const Work& w, cons
       ms::PairBuffer<D>& buffer = buffers[PARTS * parity + part];
       ms::stage_store<D, PART_THREADS>(ahead[i], thread, buffer);
       ms::stage_load<D, PART_THREADS>(ahead[i], thread, pages[i], key_pool, value_pool, page_stride, head_base, b.block_size);
-      pages[i] = ms::find_pair_pages(t + 2 * kDepth * kRound, t1, w.table, b.block_size);
+      pages[i] = ms::find_pair_pages(t + 2 * kDepth * kRound, end_tile, w.table, b.block_size);
       __syncthreads();    // the pair is in LDS; every wave is done with the other buffers' previous content
-      if (t < t1)
-        ms::consume_pair<D>(st, buffer, q_reg, t * kTileKeys, w.first_key, w.end_key - 1, w.end_key - 1, scale_log2, h,
-                            column, (t + 2) * kTileKeys > w.end_key);
+      if (t < t1) ms::consume_pair<D>(st, buffer, q_reg, t * kTileKeys, 0, 0, 0, scale_log2, h, column, false);
     }
+  }
+
+  if (t1 * kTileKeys < w.end_key) {
+    // the rest, through the first buffer of the first part
+    __syncthreads();
+    if (part == 0) {
+      ms::stage_load<D, PART_THREADS>(ahead[0], thread, ms::find_pair_pages(t1, end_tile, w.table, b.block_size), key_pool,
+                                       value_pool, page_stride, head_base, b.block_size);
+      ms::stage_store<D, PART_THREADS>(ahead[0], thread, buffers[0]);
+    }
+    __syncthreads();
+    if (part == 0)
+      ms::consume_pair<D>(st, buffers[0], q_reg, t1 * kTileKeys, w.first_key, w.end_key - 1, w.end_key - 1, scale_log2, h,
+                          column, true);
   }
 
   __syncthreads();    // everybody is done with what the memory held before
@@ -592,8 +631,11 @@ __device__ __forceinline__ void leave_empty(const Batch& b, const Work& w, int t
 // sequences' own keys, (kv head, split, tile of 16 rows, sequence) each.
 template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) void attention_shared_kernel(
-    Batch b, const T* __restrict__ q, const T* __restrict__ key_pool, const T* __restrict__ value_pool,
-    float* __restrict__ partial_o, float* __restrict__ partial_ml) {
+    Sizes sizes, const int32_t* __restrict__ block_table, const int32_t* __restrict__ query_start,
+    const int32_t* __restrict__ context_lens, const int32_t* __restrict__ group_start,
+    const int32_t* __restrict__ shared_lens, const T* __restrict__ q, const T* __restrict__ key_pool,
+    const T* __restrict__ value_pool, float* __restrict__ partial_o, float* __restrict__ partial_ml) {
+  const Batch b{sizes, block_table, query_start, context_lens, group_start, shared_lens};
   constexpr int WAVES = waves_of(ROWS);
   __shared__ __align__(16) unsigned char lds[lds_bytes<T, D, ROWS>()];
   const int per_token = b.num_q_heads / b.num_kv_heads;
@@ -756,11 +798,12 @@ int launch(const Batch& b, const void* q, const void* key_pool, const void* valu
   const int64_t items = static_cast<int64_t>((units + kXcds - 1) / kXcds * kXcds) * b.shared_tiles +
                         static_cast<int64_t>(b.num_seqs) * b.own_tiles * b.own_splits * b.num_kv_heads;
   MS_REQUIRE(items < (1LL << 31) / (8 * ms::kWave), "attention_shared_prefix: the batch is too large");
-#define MS_SHARED_ROWS(ROWS)                                                                                       \
-  hipLaunchKernelGGL((attention_shared_kernel<T, D, ROWS>), dim3(static_cast<unsigned>(items)),                 \
-                     dim3(waves_of(ROWS) * ms::kWave), 0, \
-                     stream, b, static_cast<const T*>(q), static_cast<const T*>(key_pool),                         \
-                     static_cast<const T*>(value_pool), static_cast<float*>(partial_o), static_cast<float*>(partial_ml))
+#define MS_SHARED_ROWS(ROWS)                                                                                   \
+  hipLaunchKernelGGL((attention_shared_kernel<T, D, ROWS>), dim3(static_cast<unsigned>(items)),                \
+                     dim3(waves_of(ROWS) * ms::kWave), 0, stream, static_cast<const Sizes&>(b), b.block_table, \
+                     b.query_start, b.context_lens, b.group_start, b.shared_lens, static_cast<const T*>(q),    \
+                     static_cast<const T*>(key_pool), static_cast<const T*>(value_pool),                       \
+                     static_cast<float*>(partial_o), static_cast<float*>(partial_ml))
   if constexpr (sizeof(T) == 2) {
     if (b.tile_rows == 128) MS_SHARED_ROWS(128);
     else if (b.tile_rows == 64) MS_SHARED_ROWS(64);
@@ -807,7 +850,8 @@ extern "C" int ms_attention_shared_prefix_supported(int head_dim, int block_size
 // [num_seqs + 1], context_lens [num_seqs], group_start [num_groups + 1], shared_lens
 // [num_groups]; partial_o: float [num_tokens, num_q_heads, shared_splits + own_splits,
 // head_dim]; partial_ml: the same with 2 in head_dim's place.  rows_per_tile: 16, 32, 64
-// or 128 rows of a group a workgroup (32-bit storage: 16); own_tiles: workgroups that share a sequence's tiles of 16 rows.
+// or 128 rows of a group a workgroup (32-bit storage: 16); own_tiles: workgroups that share
+// a sequence's tiles of 16 rows.
 extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, const void* value_pool,
                                           const void* block_table, const void* query_start, const void* context_lens,
                                           const void* group_start, const void* shared_lens, void* out, void* partial_o,

@@ -441,24 +441,49 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
     """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
     the parts those keys are cut into, the workgroups that share a sequence's tiles of 16
     rows, and the parts that its own keys are cut into.  ``rows``: tokens times query heads
-    of a kv head."""
+    of a kv head.
+
+    Fitted to a sweep on MI355X (head size 128, 1 to 64 sequences, 512 to 30,000 shared
+    keys, 1 to 16 groups).  Small tiles go out as workgroups of four waves, two to a compute
+    unit, and finish soonest while the chip holds them all with their fewest keys, a pair of
+    16-key tiles a wave (64 rows over 512 keys: 16 rows a tile 9.8 us, 64 rows 13.1), and where a
+    sequence's own keys are most of the work (64 sequences with 4,096 shared and 2,000 own: 32
+    rows 106 us, 64 rows 125).  Beyond that each key has to serve more rows, 64 (64 rows over
+    8,192: 18.9 us, 16 rows a tile 21.9), and 128 where a long prefix meets hundreds of rows
+    (512 over 16,384: 88 us against 104).  The units go to shared keys in proportion to their
+    work, counted in keys of a workgroup (the start of one costs as much as some 150): parts
+    that are longer than the rest of the work leave a tail, shorter ones more to join (the same
+    case in 8 parts instead of 4: 108 us)."""
 
     units = _decode_target() // 2
-    tile = 16
-    while dtype == torch.bfloat16 and tile < 128 and tile * groups < rows:
-        tile *= 2
-    tiles = max(groups, -(-rows // tile))
-    # a compute unit holds two workgroups of four waves (tiles of few rows) or one of eight;
-    # a wave has a pair of 16-key tiles at least
-    waves, room = (4, 2 * units) if tile <= 32 else (8, units)
 
-    def splits(parts: int, most: int, keys: int) -> int:
-        return max(1, min(most // parts, -(-keys // (32 * waves)), _DECODE_MAX_SPLITS))
+    def tiles(tile: int) -> int:
+        return max(groups, -(-rows // tile))
 
     own_tiles = -(-max_query * per_token // 16)
-    # groups of different lengths have their keys cut into parts of the same length: more of them, to fill the gaps
-    return (tile, splits(tiles * kv_heads, room if groups == 1 else 2 * room, max_shared), own_tiles,
-            splits(sequences * own_tiles * kv_heads, room, max_own))
+    own_parts = sequences * own_tiles * kv_heads
+    fewest_parts = -(-max_shared // 128)
+    if dtype != torch.bfloat16 or rows <= 16 or tiles(16) * kv_heads * fewest_parts < 2 * units:
+        tile = 16
+    elif tiles(32) * kv_heads * fewest_parts <= 4 * units or own_parts * max_own > 4 * tiles(64) * kv_heads * max_shared:
+        tile = 32
+    elif rows >= 256 * groups and tiles(64) * kv_heads * -(-max_shared // 256) > 8 * units:
+        tile = 128
+    else:
+        tile = 64
+    parts, few = tiles(tile) * kv_heads, tile <= 32
+    if few:
+        room = units
+    else:
+        work = parts * max_shared
+        share = work / (work + own_parts * (max_own + 150))
+        # (with little work of their own beside tiles of 128 rows the sequences' parts follow in a second turn)
+        room = units * (min(share, 0.75) if tile == 64 else share if share < 0.8 else 1)
+
+    def splits(wanted: float, keys: int) -> int:
+        return max(1, min(round(wanted), -(-keys // (128 if few else 256)), _DECODE_MAX_SPLITS))
+
+    return tile, splits(room / parts, max_shared), own_tiles, splits((2 if few else 1) * units // own_parts, max_own)
 
 
 def attention_shared_prefix(
