@@ -124,6 +124,7 @@ class _Live:
     tables: list[BlockTable] = field(default_factory=list)
     pending: bool = False
     fork: Fork | None = None
+    branched: bool = False      # took part in a fork, so that others may hold pages of its tables
 
 
 class CacheManager:
@@ -333,7 +334,7 @@ class CacheManager:
                     allocator.release(pages)
             raise
         fork = Fork(whole) if any(whole) else None
-        live.fork = fork or live.fork
+        live.fork, live.branched = fork or live.fork, True
         slots = []
         for index, child in enumerate(children):
             tables = []
@@ -344,7 +345,7 @@ class CacheManager:
                 forked.extend(pages[index : index + 1])
                 tables.append(forked)
             slot = self._free_slots.pop()
-            self._live[child] = _Live(child, slot, committed=live.committed, tables=tables, fork=fork)
+            self._live[child] = _Live(child, slot, committed=live.committed, tables=tables, fork=fork, branched=True)
             for tensor in self.state_tensors:
                 tensor[slot].copy_(tensor[live.state_slot])
             slots.append(slot)
@@ -547,7 +548,7 @@ class CacheManager:
         """Pages of each group that come free when the request goes: all it holds, but for
         those that others hold too."""
 
-        if live.fork is None:
+        if not live.branched:
             return tuple(table.live_count() for table in live.tables)
         return tuple(
             sum(allocator.refcount(page) == 1 for page in table.live_pages())

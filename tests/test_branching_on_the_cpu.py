@@ -129,6 +129,23 @@ def test_a_cut_gives_pages_back_and_copies_one_that_others_hold():
         m.truncate("q", 0)
 
 
+def test_pages_that_a_branch_would_give_back_are_those_that_it_holds_alone():
+    m = manager(num_blocks=10)
+    m.admit("p")
+    advance(m, p=10)
+    assert m.capacity().held_blocks == {"p": (3,)}
+    m.fork("p", ["x", "y"])
+    assert m.capacity().held_blocks == {"p": (1,), "x": (1,), "y": (1,)}
+    m.truncate("x", 4)          # no longer alike in all that was shared, and still on a page of the others
+    assert m.fork_of("x") is None and m.capacity().held_blocks["x"] == (0,)
+    m.release("p")
+    m.release("y")
+    assert m.capacity().held_blocks == {"x": (1,)}
+    free = m.capacity().free_blocks
+    m.release("x")
+    assert m.capacity().free_blocks == (free[0] + 1,)
+
+
 def test_a_cut_without_a_page_for_the_copy_changes_nothing():
     m = manager(num_blocks=3)
     m.admit("p")
