@@ -31,7 +31,7 @@
 //   8 rows of 32 heads over 2,048                11 us   the same
 //   45 rows of 32 heads, 7 groups of up to       39 us   161 MB in 33 us at a copy's rate; the
 //     5,000 and up to 700 keys of their own               sequences' own keys are most of it
-//   64 rows of 64 heads over 30,000              96 us   63 GFLOP: 0.66 PFLOP/s.  The products alone
+//   64 rows of 64 heads over 30,000             102 us   63 GFLOP: 0.62 PFLOP/s.  The products alone
 //                                                        take 52 us at a large product's rate, the
 //                                                        exponentials and conversions between them
 //                                                        as much again, and the waves of a unit
@@ -122,6 +122,7 @@ struct Operand<float> {
 
 struct Sizes {
   int num_tokens, num_seqs, num_groups, num_q_heads, num_kv_heads, block_size, max_blocks;
+  int most_keys;          // that a table names pages for; lengths beyond count as this
   float scale;
   int tile_rows, shared_tiles, shared_splits, own_tiles, own_splits;
 };
@@ -188,7 +189,7 @@ __device__ __forceinline__ int longest_shared(const Batch& b) {
   for (int g = lane; g < b.num_groups; g += ms::kWave) longest = max(longest, b.shared_lens[g]);
 #pragma unroll
   for (int offset = 32; offset > 0; offset >>= 1) longest = max(longest, __shfl_xor(longest, offset, ms::kWave));
-  return ms::uniform(longest);
+  return ms::uniform(min(longest, b.most_keys));
 }
 
 // The group of a sequence, -1 for one that is in none.
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) v
     if (unit >= units) return;
     const int tile = turn % b.shared_tiles, split = unit / b.num_kv_heads;
     w.kv_head = unit - split * b.num_kv_heads;
-    int group = 0, local = tile, longest = b.shared_lens[0];
+    int group = 0, local = tile, longest = min(b.shared_lens[0], b.most_keys);
     if (b.num_groups > 1) {
       longest = longest_shared(b);
       if (!find_group_tile(b, tile, per_token, ROWS, group, local)) return;
@@ -661,7 +662,7 @@ __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) v
     w.rows = (b.query_start[b.group_start[group + 1]] - w.first_token) * per_token;
     w.row0 = local * ROWS;
     if (w.row0 >= w.rows) return;
-    const int keys = max(b.shared_lens[group], 0);
+    const int keys = min(max(b.shared_lens[group], 0), b.most_keys);
     const int per_split = max((longest + b.shared_splits - 1) / b.shared_splits, split_keys(ROWS));
     const int whole_pairs = (per_split + 2 * kTileKeys - 1) / (2 * kTileKeys) * 2 * kTileKeys;
     w.first_key = min(split * whole_pairs, keys);
@@ -688,7 +689,7 @@ __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) v
   const int first_tile = item % b.own_tiles;
   const int seq = item / b.own_tiles;
   const int group = b.num_groups > 1 ? group_of_sequence(b, seq) : seq >= b.group_start[0] && seq < b.group_start[1] ? 0 : -1;
-  const int context = max(b.context_lens[seq], 0);
+  const int context = min(max(b.context_lens[seq], 0), b.most_keys);
   w.first_token = b.query_start[seq];
   const int tokens = b.query_start[seq + 1] - w.first_token;
   w.rows = tokens * per_token;
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) v
 }
 
 // Joins the parts of a row, a wave each.  A row that saw no key gives zeros, and so do the
-// rows of tokens behind the last sequence.
+// rows of tokens before the first sequence and behind the last.
 constexpr int kJoinWaves = 4;
 
 template <typename T, int D>
@@ -742,7 +743,8 @@ __global__ __launch_bounds__(kJoinWaves * ms::kWave) void attention_shared_join_
 #pragma unroll
   for (int u = 0; u < kDeep; ++u)
     ahead[u] = *reinterpret_cast<const floatx4*>(from + static_cast<int64_t>(min(group + u * kAtOnce, slots - 1)) * D);
-  const bool live = row / num_q_heads < query_start[num_seqs];
+  const int64_t token = row / num_q_heads;
+  const bool live = token >= query_start[0] && token < query_start[num_seqs];
   float m[2], mx = -INFINITY, l[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -890,6 +892,8 @@ extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, c
   b.num_kv_heads = num_kv_heads;
   b.block_size = block_size;
   b.max_blocks = max_blocks;
+  const int64_t named = static_cast<int64_t>(max_blocks) * block_size;
+  b.most_keys = named < (1LL << 30) ? static_cast<int>(named) : 1 << 30;
   b.scale = scale;
   // every group has at most one tile that is not full
   b.tile_rows = rows_per_tile;

@@ -517,7 +517,8 @@ def attention_shared_prefix(
     ``max_shared``, ``max_own`` (keys behind the shared ones) and ``max_query`` (tokens a
     sequence brings) say how long things are at most, for the cut of the work; results do
     not hang on them beyond rounding.  A token that sees no key gives zeros, as do rows of
-    ``q`` behind the last sequence.  The caller guarantees that every page that the tables
+    ``q`` before the first sequence and behind the last.  Lengths beyond what a table's row
+    names pages for count as that.  The caller guarantees that every page that the tables
     name for the keys that are read lies inside the pool.
 
     Takes float32 and bfloat16, head sizes in steps of 16 up to 128 and pages of a multiple
@@ -589,6 +590,9 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
             raise KernelError(f"copy_pages: pools[{index}] {tuple(pool.shape)} is not [calls>0, pages>0, ...].")
         at = _address(pool, f"pools[{index}]", torch.cuda.current_device(), pool.dtype)
         described.append((at, pool.stride(1) * pool.element_size(), pool.shape[0], pool.shape[1]))
+    ends = sorted((at, at + calls * pages * page_bytes) for at, page_bytes, calls, pages in described)
+    if any(after[0] < before[1] for before, after in zip(ends, ends[1:])):
+        raise KernelError("copy_pages: two pools lie in the same memory.")
     count = len(source)
     if len(destination) != count:
         raise KernelError(f"copy_pages: {count} pages to {len(destination)} places.")

@@ -164,6 +164,23 @@ def test_empty_groups_sequences_and_rows(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_lengths_beyond_a_table_count_as_its_keys_and_rows_before_the_first_sequence_are_zero(ops, dtype):
+    case = attention_case(dtype, 8, 4, 64, 16, [(64, [(1, 16), (1, 16)])], alone=[(1, 80)])
+    case["block_table"] = case["block_table"][:, :5].contiguous()
+    check_attention(ops, case)
+    far = {**case, "context_lens": ints([10**6, 2**31 - 1, 81])}
+    again = ops.attention_shared_prefix(**far, max_own=16)
+    # (bounds only move rounding, and here they cut the work alike)
+    assert torch.equal(again, ops.attention_shared_prefix(**case, max_own=16))
+    same = case["block_table"].clone()
+    same[1] = same[0]
+    check_attention(ops, {**case, "block_table": same, "shared_lens": ints([2**31 - 1])})
+    later = {**case, "q": torch.cat([case["q"][:2], case["q"]]), "query_start": case["query_start"] + 2}
+    moved = ops.attention_shared_prefix(**later)
+    assert not bool(moved[:2].any()) and torch.equal(moved[2:], ops.attention_shared_prefix(**case))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_parts_are_split_and_joined(ops, dtype):
     check_attention(ops, attention_case(dtype, 4, 1, 64, 64, [(3000, [(1, 2100), (1, 1)])], seed=2))
     check_attention(ops, attention_case(dtype, 8, 2, 32, 16, [(1600, [(1, 1 + i) for i in range(40)])], seed=2))
@@ -530,7 +547,8 @@ def test_refusals_of_the_gpu_side(ops):
         ("outside", [pool, torch.zeros(2, 3, 8, device=DEVICE)], [4], [1]), ("two copies", [pool], [0, 1], [2, 2]),
         ("source of one copy", [pool], [0, 1], [1, 2]), ("source of one copy", [pool], [3], [3]), ("1 pages to 2", [pool], [0], [1, 2]),
         ("whole numbers", [pool], [0.0], [1]), ("whole numbers", [pool], [True], [2]), ("contiguous", [pool[:, :, ::2]], [0], [1]),
-        ("calls>0", [torch.zeros(5, device=DEVICE)], [0], [1]),
+        ("calls>0", [torch.zeros(5, device=DEVICE)], [0], [1]), ("same memory", [pool, pool], [0], [1]),
+        ("same memory", [pool[1:], pool.view(1, 10, 8)], [0], [1]),
     ]:
         with pytest.raises(KernelError, match=match):
             ops.copy_pages(pools, source, destination)
