@@ -41,28 +41,53 @@ class StepEntry:
             raise ValueError(f"entry {self.request_id!r}: wanted places must index its tokens.")
 
 
-# A step reads common pages of forked requests once (ops.attention_shared_prefix) from this
-# many keys on, and where no request brings more than SHARED_FRONT_TOKENS tokens (a decoded
-# token, or one with drafted ones behind it): prompts go to the tiled kernel.
-SHARED_FRONT_KEYS = 256
+# A step reads common pages of forked requests once (ops.attention_shared_prefix) where some
+# share at least this many keys and at least half of all keys that the rows see need not be
+# read again, and where no request brings more than SHARED_FRONT_TOKENS tokens (a decoded token, or
+# one with drafted ones behind it): prompts go to the tiled kernel.  Measured on MI355X with 2
+# to 64 single tokens, head size 128, 8 kv heads, against each row reading its own keys: with
+# 1,024 shared keys and half or more spared the kernel takes 0.94 of the time at most and 0.5
+# at best (64 rows: 15.2 us against 30.5), with 256 keys 1 to 1.2 of it, and pairs, which
+# spare less than half, 0.9 to 1.3 up to 1,024 keys.
+SHARED_FRONT_KEYS = 512
 SHARED_FRONT_TOKENS = 16
 
 
-def shared_fronts(forks: Sequence[Fork | None], group: int, block_size: int) -> tuple[list[int], list[int]] | None:
-    """The step's sequences, in the order of its rows, as runs of neighbours of one fork:
-    where each run begins (and the end of the last), and the keys that it shares (0 for a
-    sequence alone).  None when no run shares ``SHARED_FRONT_KEYS``."""
+@dataclass(frozen=True)
+class Fronts:
+    """The step's sequences as groups of neighbours, as ops.attention_shared_prefix takes them
+    (sequences behind the last group share nothing)."""
 
-    starts, lens, pays = [0], [], False
-    for row, fork in enumerate(forks):
-        if row > 0 and fork is not None and fork is forks[row - 1]:
-            lens[-1] = fork.pages[group] * block_size
-            pays = pays or lens[-1] >= SHARED_FRONT_KEYS
-            starts[-1] = row + 1
+    starts: list[int]      # where each group begins, and the end of the last
+    lens: list[int]        # keys that it shares, 0 for neighbours that share nothing
+    runs: int              # groups that share keys; there are at most twice as many groups
+    behind: int            # most keys of a sequence that it does not share
+
+
+def shared_fronts(forks: Sequence[Fork | None], contexts: Sequence[int], group: int, block_size: int) -> Fronts | None:
+    """What the step's sequences share with their neighbours: those of one fork side by side
+    share its pages.  ``contexts``: their lengths after the step.  None where it does not pay."""
+
+    starts, lens, runs, spared, behind, row = [0], [], 0, 0, 0, 0
+    while row < len(forks):
+        fork, end = forks[row], row + 1
+        while fork is not None and end < len(forks) and forks[end] is fork:
+            end += 1
+        length = fork.pages[group] * block_size if end > row + 1 else 0
+        if length == 0 and lens and lens[-1] == 0:
+            starts[-1] = end
         else:
-            starts.append(row + 1)
-            lens.append(0)
-    return (starts, lens) if pays else None
+            starts.append(end)
+            lens.append(length)
+        runs += length > 0
+        spared += (end - row - 1) * length
+        behind = max(behind, max(contexts[row:end]) - length)
+        row = end
+    if not runs or max(lens) < SHARED_FRONT_KEYS or 2 * spared < sum(contexts):
+        return None
+    if lens[-1] == 0:
+        del starts[-1], lens[-1]
+    return Fronts(starts, lens, runs, behind)
 
 
 @dataclass
@@ -140,10 +165,11 @@ def build_step(
     num_rows = sum(len(entry.want) for entry in entries)
     widest = [max(1, max(len(meta.block_tables[group]) for meta in metas_in_layout)) for group in range(num_groups)]
 
-    fronts: list[tuple[list[int], list[int]] | None] = [None] * num_groups
+    fronts: list[Fronts | None] = [None] * num_groups
     forks = [getattr(meta, "fork", None) for meta in metas_in_layout]
     if any(fork is not None for fork in forks) and max(query_lens) <= SHARED_FRONT_TOKENS:
-        fronts = [shared_fronts(forks, group, block_sizes[group]) for group in range(num_groups)]
+        contexts = [meta.after for meta in metas_in_layout]
+        fronts = [shared_fronts(forks, contexts, group, block_sizes[group]) for group in range(num_groups)]
 
     offsets: dict[str, tuple[int, int]] = {}
     total = 0
@@ -151,7 +177,7 @@ def build_step(
              ("state_slots", s), ("logit_rows", num_rows)]
     for group, front in enumerate(fronts):
         if front is not None:
-            sizes += [(f"front_start{group}", len(front[0])), (f"front_lens{group}", len(front[1]))]
+            sizes += [(f"front_start{group}", len(front.starts)), (f"front_lens{group}", len(front.lens))]
     sizes += [(f"part:{name}", values.size) for name, values in part_tables.items()]
     for group in range(num_groups):
         sizes += [(f"slots{group}", n), (f"table{group}", s * widest[group])]
@@ -238,7 +264,7 @@ def build_step(
         region(f"part:{name}")[:] = values
     for group, front in enumerate(fronts):
         if front is not None:
-            region(f"front_start{group}")[:], region(f"front_lens{group}")[:] = front
+            region(f"front_start{group}")[:], region(f"front_lens{group}")[:] = front.starts, front.lens
     buffer = torch.empty(total, dtype=torch.int32, device=device) if on_gpu else host
 
     def view(name: str) -> torch.Tensor:
@@ -249,9 +275,8 @@ def build_step(
         front = fronts[group]
         if front is None:
             return None
-        behind = max(context_lens[row] - length for first, end, length in zip(front[0], front[0][1:], front[1])
-                     for row in range(first, end))
-        return SharedFronts(view(f"front_start{group}"), view(f"front_lens{group}"), max(front[1]), behind, max(query_lens))
+        return SharedFronts(view(f"front_start{group}"), view(f"front_lens{group}"), front.runs, max(front.lens), front.behind,
+                            max(query_lens))
 
     groups = [
         GroupStepView(block_table=view(f"table{g}").view(s, widest[g]), slot_mapping=view(f"slots{g}"), shared=shared_view(g))

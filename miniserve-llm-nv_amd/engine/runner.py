@@ -77,11 +77,12 @@ class DecodeGraph:
     whose state slot is the spare slot.  They write and read nothing that a request
     holds, and their logits are not returned.
 
-    ``shared``: a recording for steps with neighbouring rows of forked requests; where those
-    runs lie and how many keys they share is among the step's numbers.
+    ``shared``: of a recording for steps with neighbouring rows of forked requests, the most
+    runs of them and the most keys that a row does not share; where the runs lie and how
+    many keys they share is among the step's numbers.
     """
 
-    def __init__(self, runner: "ModelRunner", batch: int, bound: int, shared: bool = False) -> None:
+    def __init__(self, runner: "ModelRunner", batch: int, bound: int, shared: tuple[int, int] | None = None) -> None:
         self.batch = batch
         self.bound = bound
         self.shared = shared
@@ -99,8 +100,8 @@ class DecodeGraph:
         sizes += [(f"part:{name}", values.size) for name, values in part_tables.items()]
         for group in range(groups):
             sizes += [(f"slots{group}", batch), (f"table{group}", batch * widths[group])]
-            if shared:
-                sizes += [(f"front_start{group}", batch + 1), (f"front_lens{group}", batch)]
+            if shared is not None:
+                sizes += [(f"front_start{group}", 2 * shared[0] + 1), (f"front_lens{group}", 2 * shared[0])]
         # for a step launched behind the sampling of the step before: which of that step's rows each row continues
         sizes += [("token_rows", batch)]
         self.offsets: dict[str, tuple[int, int]] = {}
@@ -131,7 +132,8 @@ class DecodeGraph:
             state_slots=view("state_slots"),
             groups=[
                 GroupStepView(block_table=view(f"table{g}").view(batch, widths[g]), slot_mapping=view(f"slots{g}"),
-                              shared=SharedFronts(view(f"front_start{g}"), view(f"front_lens{g}"), bound, bound, 1) if shared else None)
+                              shared=None if shared is None else SharedFronts(
+                                  view(f"front_start{g}"), view(f"front_lens{g}"), shared[0], bound, shared[1], 1))
                 for g in range(groups)
             ],
             # what holds for every replay: one token a row.  Launch decisions inside the
@@ -181,13 +183,14 @@ class DecodeGraph:
         put("context_lens", [meta.after for meta in metas] + [1] * spare)
         put("state_slots", [meta.state_slot for meta in metas] + [runner.cache.spare_state_slot] * spare)
         put("logit_rows", range(batch))
-        forks = [meta.fork for meta in metas]
+        forks, contexts = [meta.fork for meta in metas], [meta.after for meta in metas]
         for group in range(len(runner.cache.layout.groups)):
-            if self.shared:
-                # rows in no run, and runs that are not there, share nothing
-                starts, lens = shared_fronts(forks, group, runner.cache.block_sizes[group]) or ([0], [])
-                put(f"front_start{group}", starts + [starts[-1]] * (batch + 1 - len(starts)))
-                put(f"front_lens{group}", lens + [0] * (batch - len(lens)))
+            if self.shared is not None:
+                # groups that are not there, and rows in none, share nothing
+                fronts = shared_fronts(forks, contexts, group, runner.cache.block_sizes[group])
+                starts, lens = (fronts.starts, fronts.lens) if fronts is not None else ([0], [])
+                put(f"front_start{group}", starts + [starts[-1]] * (2 * self.shared[0] + 1 - len(starts)))
+                put(f"front_lens{group}", lens + [0] * (2 * self.shared[0] - len(lens)))
             pool_pages = runner.cache.num_blocks[group]
             block_size, width = runner.cache.block_sizes[group], self.widths[group]
             slots = []
@@ -354,7 +357,7 @@ class ModelRunner:
         )
         self.cache.allocate_storage(self.dtype, self.device)
         self._call_views = self.cache.call_views()
-        self._decode_graphs: dict[tuple, DecodeGraph] = {}     # by (rows, context bound), and True for steps with shared fronts
+        self._decode_graphs: dict[tuple, DecodeGraph] = {}     # by ``_recorded_step_key``
         self._graph_pool = None
         self.steps_run = 0
         self.tokens_run = 0
@@ -410,23 +413,32 @@ class ModelRunner:
         blocks = max(1, min(by_memory, by_need))
         return blocks
 
-    def _recorded_step_key(self, longest: int, forks: Sequence) -> tuple:
+    def _recorded_step_key(self, contexts: Sequence[int], forks: Sequence) -> tuple:
         """(rows, context bound) of the recorded step that serves a single token for each of
-        ``forks`` (the requests' ``Fork`` or None), the longest row of which has ``longest``
-        tokens after the step; with True behind them for a step that reads common pages of
-        neighbouring rows once."""
+        the requests, ``contexts`` their lengths after the step and ``forks`` their ``Fork``
+        or None; for a step that reads common pages of neighbouring rows once, with the
+        most runs of such rows (1, 2, 4, ...) and the most keys that a row does not share
+        (256, 1024, 4096, ...) behind them: the kernel's launch is cut by both."""
 
-        key = recorded_batch_size(len(forks)), recorded_context_bound(longest, self.max_model_len)
-        if self.dtype == torch.bfloat16 and any(fork is not None for fork in forks) and any(
-            group.window is None and shared_fronts(forks, group.index, self.cache.block_sizes[group.index])
-            for group in self.cache.layout.groups
-        ):
-            key += (True,)
-        return key
+        bound = recorded_context_bound(max(contexts), self.max_model_len)
+        key = recorded_batch_size(len(forks)), bound
+        if self.dtype != torch.bfloat16 or all(fork is None for fork in forks):
+            return key
+        fronts = [shared_fronts(forks, contexts, group.index, self.cache.block_sizes[group.index])
+                  for group in self.cache.layout.groups if group.window is None]
+        fronts = [front for front in fronts if front is not None]
+        if not fronts:
+            return key
+        runs, behind = 1, 256
+        while runs < max(front.runs for front in fronts):
+            runs *= 2
+        while behind < max(front.behind for front in fronts):
+            behind *= 4
+        return (*key, (runs, min(behind, bound)))
 
     def _recorded_step_key_of(self, reservation) -> tuple:
         metas = reservation.sequences
-        return self._recorded_step_key(max(meta.after for meta in metas), [meta.fork for meta in metas])
+        return self._recorded_step_key([meta.after for meta in metas], [meta.fork for meta in metas])
 
     def _decode_graph_step(self, entries: Sequence[StepEntry], reservation, prepared: int | None = None) -> torch.Tensor | None:
         """A step of single tokens through the recorded graph of its batch size.  The
@@ -494,7 +506,7 @@ class ModelRunner:
             start = self.cache.committed_tokens(request_id)
             items.append(StepItem(request_id, start, start + 1))
         graph = self._decode_graphs.get(self._recorded_step_key(
-            max(item.end for item in items), [self.cache.fork_of(request_id) for request_id in request_ids]))
+            [item.end for item in items], [self.cache.fork_of(request_id) for request_id in request_ids]))
         if graph is None or graph.graph is None:
             return None
         reservation = self.cache.prepare_step(items)

@@ -441,7 +441,7 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
     """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
     the parts those keys are cut into, the workgroups that share a sequence's tiles of 16
     rows, and the parts that its own keys are cut into.  ``rows``: tokens times query heads
-    of a kv head.
+    of a kv head; ``groups``: those that share keys.
 
     Fitted to a sweep on MI355X (head size 128, 1 to 64 sequences, 512 to 30,000 shared
     keys, 1 to 16 groups).  Small tiles go out as workgroups of four waves, two to a compute
@@ -497,6 +497,7 @@ def attention_shared_prefix(
     group_start: torch.Tensor,
     shared_lens: torch.Tensor,
     scale: float,
+    max_sharing: int | None = None,
     max_shared: int | None = None,
     max_own: int | None = None,
     max_query: int | None = None,
@@ -514,9 +515,10 @@ def attention_shared_prefix(
     empty.  All four are int32 on the device, so that a recorded graph serves other
     lengths and groups of the same sizes on every replay.
 
-    ``max_shared``, ``max_own`` (keys behind the shared ones) and ``max_query`` (tokens a
-    sequence brings) say how long things are at most, for the cut of the work; results do
-    not hang on them beyond rounding.  A token that sees no key gives zeros, as do rows of
+    ``max_sharing`` (groups that share keys), ``max_shared``, ``max_own`` (keys behind the
+    shared ones) and ``max_query`` (tokens a sequence brings) say how many there are and how
+    long things are at most, for the cut of the work; results do not hang on them beyond
+    rounding.  A token that sees no key gives zeros, as do rows of
     ``q`` before the first sequence and behind the last.  Lengths beyond what a table's row
     names pages for count as that.  The caller guarantees that every page that the tables
     name for the keys that are read lies inside the pool.
@@ -554,12 +556,12 @@ def attention_shared_prefix(
     shared_at = _address(shared_lens, "shared_lens", device, torch.int32, (groups,))
     longest = max_blocks * block_size
     bounds = []
-    for name, given, most in (("max_shared", max_shared, longest), ("max_own", max_own, longest), ("max_query", max_query, n)):
+    for name, given, most in (("max_sharing", max_sharing, groups), ("max_shared", max_shared, longest), ("max_own", max_own, longest), ("max_query", max_query, n)):
         if given is not None and (type(given) is not int or given < 0):
             raise KernelError(f"attention_shared_prefix: {name} must be a whole number or None, not {given!r}.")
         bounds.append(max(1, most if given is None else min(given, most)))
     per_token = heads // kv_heads
-    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, groups, sequences, kv_heads, per_token, *bounds, dtype)
+    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, bounds[0], sequences, kv_heads, per_token, *bounds[1:], dtype)
     out = torch.empty_like(q)
     # of every part of a row's keys the outputs, then the maximum and the sum
     parts = n * heads * (shared_splits + own_splits)

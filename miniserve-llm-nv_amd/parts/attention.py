@@ -181,6 +181,7 @@ class Attention(Part):
                 group_start=shared.group_start,
                 shared_lens=shared.shared_lens,
                 scale=self.scale,
+                max_sharing=shared.max_sharing,
                 max_shared=shared.max_shared,
                 max_own=shared.max_own,
                 max_query=shared.max_query,

@@ -155,11 +155,13 @@ class StateView:
 class SharedFronts:
     """Runs of neighbouring sequences whose block tables begin with the same pages: group
     ``g`` is the sequences ``group_start[g] .. group_start[g + 1] - 1``, which share their
-    first ``shared_lens[g]`` keys.  The bounds hold for every replay of a recorded step."""
+    first ``shared_lens[g]`` keys (0: none).  The bounds are those of every replay of a
+    recorded step."""
 
     group_start: torch.Tensor    # int32 [groups + 1]
     shared_lens: torch.Tensor    # int32 [groups]
-    max_shared: int
+    max_sharing: int             # groups that share keys
+    max_shared: int              # keys that one shares
     max_own: int                 # keys behind the shared ones
     max_query: int               # tokens that a sequence brings
 

@@ -291,6 +291,9 @@ def make_runner(folder, block_size, dtype, **options):
 @pytest.mark.parametrize("recorded", [False, True], ids=["eager", "recorded"])
 @pytest.mark.parametrize("name,dtype", [("a", "float32"), ("a", "bfloat16"), ("b", "bfloat16"), ("c", "bfloat16")])
 def test_branches_follow_the_plain_implementation(name, dtype, recorded, model_folders, monkeypatch):
+    from miniserve_amd.engine import batch
+
+    monkeypatch.setattr(batch, "SHARED_FRONT_KEYS", 256)       # the plain implementation takes its time over longer prompts
     kernels.install(monkeypatch, recordings=recorded)
     folder, block_size = model_folders[name]
     runner = make_runner(folder, block_size, dtype, decode_graphs=recorded)
@@ -308,13 +311,34 @@ def test_branches_follow_the_plain_implementation(name, dtype, recorded, model_f
 
 def test_runs_of_neighbours():
     from miniserve_amd.cache import Fork
-    from miniserve_amd.engine.batch import shared_fronts
+    from miniserve_amd.engine.batch import Fronts, shared_fronts
 
-    f, g = Fork((20, 3)), Fork((16, 40))
-    assert shared_fronts([f, f, None, g, f, g, g], 0, 16) == ([0, 2, 3, 4, 5, 7], [320, 0, 0, 0, 256])
-    assert shared_fronts([f, None, f, g], 0, 16) is None                     # nobody next to its like
-    assert shared_fronts([f, f], 1, 16) is None                              # 48 keys: too few to pay
-    assert shared_fronts([None, None], 0, 16) is None and shared_fronts([], 0, 16) is None
+    f, g = Fork((40, 3)), Fork((32, 40))
+    #                       rows 0 and 1 share 640 keys, 2 to 4 nothing with a neighbour, 5 to 7 share 512
+    contexts = [650, 660, 9, 20, 41, 600, 700, 530]
+    assert shared_fronts([f, f, None, g, f, g, g, g], contexts, 0, 16) == Fronts([0, 2, 5, 8], [640, 0, 512], 2, 188)
+    assert shared_fronts([None, f, f, f, None, g], [5, 641, 642, 643, 9, 7], 0, 16) == Fronts([0, 1, 4], [0, 640], 1, 9)
+    assert shared_fronts([f, None, f, g], [641, 1, 641, 513], 0, 16) is None       # nobody next to its like
+    assert shared_fronts([f, f, f], [50, 50, 50], 1, 16) is None                   # 48 keys: too few to pay
+    assert shared_fronts([f, f], [641, 641], 0, 16) is None                        # less than half is spared
+    assert shared_fronts([None, None], [900, 900], 0, 16) is None and shared_fronts([], [], 0, 16) is None
+    rng = random.Random(3)
+    for _ in range(300):
+        forks = [rng.choice([None, f, f, g]) for _ in range(rng.randint(1, 20))]
+        contexts = [rng.randint(641, 660) for _ in forks]
+        fronts = shared_fronts(forks, contexts, 0, 16)
+        if fronts is None:
+            continue
+        assert fronts.starts[0] == 0 and len(fronts.starts) == len(fronts.lens) + 1 <= 2 * fronts.runs + 1
+        assert sum(length > 0 for length in fronts.lens) == fronts.runs and fronts.starts[-1] <= len(forks)
+        shares = [0] * len(forks)
+        for first, end, length in zip(fronts.starts, fronts.starts[1:], fronts.lens):
+            assert end > first and (length == 0 or len({id(fork) for fork in forks[first:end]}) == 1)
+            shares[first:end] = [length] * (end - first)
+        for row, fork in enumerate(forks):
+            like = fork is not None and any(0 <= near < len(forks) and forks[near] is fork for near in (row - 1, row + 1))
+            assert shares[row] == (fork.pages[0] * 16 if like else 0)
+        assert fronts.behind == max(context - length for context, length in zip(contexts, shares))
 
 
 # ---- drafted tokens through the sampler ----------------------------------------------------

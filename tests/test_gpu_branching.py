@@ -25,9 +25,11 @@ def make_runner(folder, block_size, dtype, recorded):
 
 @pytest.mark.parametrize("recorded", [False, True], ids=["eager", "recorded"])
 @pytest.mark.parametrize("name,dtype", [("a", "float32"), ("a", "bfloat16"), ("b", "bfloat16"), ("c", "float32"), ("c", "bfloat16")])
-def test_branches_follow_the_plain_implementation(name, dtype, recorded, model_folders):
+def test_branches_follow_the_plain_implementation(name, dtype, recorded, model_folders, monkeypatch):
     from miniserve_amd import ops
+    from miniserve_amd.engine import batch
 
+    monkeypatch.setattr(batch, "SHARED_FRONT_KEYS", 256)       # the plain implementation takes its time over longer prompts
     folder, block_size = model_folders[name]
     config = read_config(folder)
     before = dict(ops.attention_calls)

@@ -189,8 +189,8 @@ def test_long_parts_are_split_and_joined(ops, dtype):
 def test_bounds_that_are_too_small_or_missing_change_nothing_but_speed(ops):
     case = attention_case(torch.bfloat16, 8, 2, 64, 16, [(320, [(9, 40), (20, 333), (1, 1)]), (16, [(3, 80)])], seed=1)
     check_attention(ops, case)
-    check_attention(ops, case, max_shared=1, max_own=1, max_query=1)
-    check_attention(ops, case, max_shared=10**6, max_own=10**6, max_query=10**6)
+    check_attention(ops, case, max_sharing=0, max_shared=1, max_own=1, max_query=1)
+    check_attention(ops, case, max_sharing=10**6, max_shared=10**6, max_own=10**6, max_query=10**6)
     check_attention(ops, case, max_shared=320, max_own=333, max_query=20)
 
 
@@ -531,6 +531,7 @@ def test_refusals_of_the_gpu_side(ops):
     refused("shared_lens must have shape", shared_lens=ints([32, 32]))
     refused("at least one group", group_start=ints([0]), shared_lens=ints([]))
     refused("whole number", max_shared=-1)
+    refused("whole number", max_sharing=True)
     refused("whole number", max_query=1.5)
     odd = attention_case(torch.bfloat16, 8, 2, 64, 16, [(32, [(1, 4)])])
     with pytest.raises(KernelError, match="head_dim 8"):

@@ -11,7 +11,7 @@ CALLS = {"attention_shared_prefix": 0, "copy_pages": 0, "verify_drafts": 0}
 
 
 def attention_shared_prefix(q, key_pool, value_pool, *, block_table, query_start, context_lens, group_start, shared_lens, scale,
-                            max_shared=None, max_own=None, max_query=None):
+                            max_sharing=None, max_shared=None, max_own=None, max_query=None):
     """Each sequence over its own table, but the keys that its group shares over the table of
     the group's first sequence, and with the contract checked."""
 
@@ -19,6 +19,7 @@ def attention_shared_prefix(q, key_pool, value_pool, *, block_table, query_start
     page, table = key_pool.shape[2], block_table.clone()
     starts = group_start.tolist()
     assert starts == sorted(starts) and 0 <= starts[0] and starts[-1] <= block_table.shape[0]
+    assert sum(length > 0 for length in shared_lens.tolist()) <= max_sharing
     for g, length in enumerate(shared_lens.tolist()):
         rows = range(starts[g], starts[g + 1])
         assert length % page == 0 and length <= max_shared
