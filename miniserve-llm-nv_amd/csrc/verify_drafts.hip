@@ -573,8 +573,10 @@ extern "C" int ms_verify_drafts(const void* logits, const void* row_start, const
                      dim3(kRowThreads), 0, stream, b, parts);
   MS_CHECK_LAUNCH("verify_drafts (rows)");
   const dim3 grid(b.chunks, requests);
-  // decisions apart where the workgroups of (2) do not all run at once
-  if (static_cast<int64_t>(b.chunks) * requests > 2 * ms_compute_units()) {
+  // decisions apart where the workgroups of (2) run in several turns (vocabulary 151,936, all
+  // kernels: 64 requests of 8 drafts 108 us apart and 115 together, 32 of 4 the same, 16 of 4
+  // 35.5 and 33.0, one 19.9 and 18.2)
+  if (static_cast<int64_t>(b.chunks) * requests > 4 * ms_compute_units()) {
     hipLaunchKernelGGL(verify_decide_kernel, dim3(requests), dim3(kChooseThreads), 0, stream, b,
                        static_cast<const RowPart*>(parts), decisions);
     MS_CHECK_LAUNCH("verify_drafts (decide)");

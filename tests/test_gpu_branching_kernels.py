@@ -405,6 +405,17 @@ def test_verify_drafts_temperatures(ops, temperature):
         check_verify(ops, draft_case([2, 5, 0, 1, 7, 3, 3], 5003, temperature=temperature, seed=seed, probs=seed % 2 == 0))
 
 
+@pytest.mark.parametrize("requests,vocab", [(1100, 130), (400, 9001)])
+def test_verify_drafts_of_many_requests(ops, requests, vocab):
+    rng = random.Random(vocab)
+    drafts = [rng.randint(0, 4) for _ in range(requests)]
+    case = draft_case(drafts, vocab, temperature=[rng.choice([0.0, 0.7, 1.0]) for _ in drafts], seed=requests)
+    for request in (3, requests - 1):      # these end with -1, at the first row that is reached
+        case["logits"][int(case["row_start"][request])] = float("nan")
+    taken = check_verify(ops, case)
+    assert sum(taken) > requests // 2
+
+
 def test_verify_drafts_greedy_and_sampled_requests_in_one_call(ops):
     case = draft_case([3, 3, 3, 0, 0, 6], 7001, temperature=[0.0, 0.7, 0.0, 0.0, 1.0, 0.0], agree=0.05, seed=2)
     taken = check_verify(ops, case)
