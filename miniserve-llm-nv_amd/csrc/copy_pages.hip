@@ -1,6 +1,6 @@
 // Copies of whole cache pages inside their pools, in every call (layer) at once: pool[c,
 // destination[i]] = pool[c, source[i]] for all c and i.  Sources and destinations are
-// disjoint and the destinations distinct (the caller checks), so the copies may run in any
+// disjoint and the destinations distinct (checked below), so the copies may run in any
 // order; one source may have several destinations.
 //
 // The page numbers travel with the launch itself, as its arguments: a table in device
@@ -12,6 +12,8 @@
 // Measured on MI355X (pages of 16 keys, 8 kv heads of 128, bf16): 1,000 pages in 28 layers,
 // 3.7 GB read and written, 700 us = 5.2 TB/s (a large copy in one piece: 4.9); 48 pages in 36
 // layers 35 us; one page in 28 layers 3 us.
+#include <cstdlib>
+
 #include "common.hpp"
 
 namespace {
@@ -82,6 +84,8 @@ extern "C" int ms_copy_pages_most_pools() { return kPools; }
 
 // bases, page_bytes, calls, pages: one entry a pool [calls, pages, page_bytes]; source,
 // destination: `count` page numbers each.  All in host memory, read before the call returns.
+// (What the numbers must be is checked here, before anything is launched: for some hundred pages
+// a check in Python takes longer than the copy.)
 extern "C" int ms_copy_pages(const void* const* bases, const int64_t* page_bytes, const int32_t* calls,
                              const int32_t* pages, int num_pools, const int32_t* source, const int32_t* destination,
                              int count, hipStream_t stream) {
@@ -89,7 +93,7 @@ extern "C" int ms_copy_pages(const void* const* bases, const int64_t* page_bytes
   MS_REQUIRE(count >= 1, "copy_pages: no pages");
   Pool described[kPools] = {};
   int64_t most_bytes = 0;
-  int32_t most_calls = 0;
+  int32_t most_calls = 0, fewest_pages = 0;
   uint64_t alignment = 0;
   for (int p = 0; p < num_pools; ++p) {
     MS_REQUIRE(bases[p] != nullptr && page_bytes[p] > 0 && calls[p] > 0 && calls[p] <= 65535 && pages[p] > 0,
@@ -98,10 +102,23 @@ extern "C" int ms_copy_pages(const void* const* bases, const int64_t* page_bytes
     most_bytes = page_bytes[p] > most_bytes ? page_bytes[p] : most_bytes;
     most_calls = calls[p] > most_calls ? calls[p] : most_calls;
     alignment |= reinterpret_cast<uint64_t>(bases[p]) | static_cast<uint64_t>(page_bytes[p]);
-    for (int i = 0; i < count; ++i)
-      MS_REQUIRE(source[i] >= 0 && source[i] < pages[p] && destination[i] >= 0 && destination[i] < pages[p],
-                 "copy_pages: page %d or %d lies outside the pool's %d", source[i], destination[i], pages[p]);
+    fewest_pages = p == 0 || pages[p] < fewest_pages ? pages[p] : fewest_pages;
   }
+  for (int i = 0; i < count; ++i)
+    MS_REQUIRE(source[i] >= 0 && source[i] < fewest_pages && destination[i] >= 0 && destination[i] < fewest_pages,
+               "copy_pages: page %d or %d lies outside the pools' %d", source[i], destination[i], fewest_pages);
+  int twice = -1, both = -1;
+  uint8_t* written = static_cast<uint8_t*>(calloc(fewest_pages, 1));
+  MS_REQUIRE(written != nullptr, "copy_pages: no memory for a list of %d pages", fewest_pages);
+  for (int i = 0; i < count; ++i) {
+    if (written[destination[i]]) twice = destination[i];
+    written[destination[i]] = 1;
+  }
+  for (int i = 0; i < count; ++i)
+    if (written[source[i]]) both = source[i];
+  free(written);
+  MS_REQUIRE(twice < 0, "copy_pages: page %d is the destination of two copies", twice);
+  MS_REQUIRE(both < 0, "copy_pages: page %d is the source of one copy and the destination of another", both);
   const int word = alignment % 16 == 0 ? 16 : alignment % 4 == 0 ? 4 : 1;
   const int64_t per_group = static_cast<int64_t>(word) * kThreads * kUnroll;
   const int64_t chunks = (most_bytes + per_group - 1) / per_group;

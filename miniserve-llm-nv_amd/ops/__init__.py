@@ -6,6 +6,7 @@ torch is the allocator and gives the stream.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import dataclasses
@@ -602,22 +603,19 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
         return
     if {*map(type, source), *map(type, destination)} != {int}:
         raise KernelError("copy_pages: pages are named by whole numbers.")
-    fewest = min(pages for *_, pages in described)
-    if min(source) < 0 or max(source) >= fewest or min(destination) < 0 or max(destination) >= fewest:
-        raise KernelError(f"copy_pages: a page lies outside the pools' {fewest}.")
-    places = set(destination)
-    if len(places) != count:
-        raise KernelError("copy_pages: a page is the destination of two copies.")
-    if not places.isdisjoint(source):
-        raise KernelError("copy_pages: a page is the source of one copy and the destination of another.")
-    numbers = (ctypes.c_int32 * count)
-    from_pages, to_pages = numbers(*source), numbers(*destination)
+    try:
+        from_pages, to_pages = array.array("i", source), array.array("i", destination)
+    except OverflowError:
+        raise KernelError("copy_pages: a page lies outside the pools.") from None
     most = int(load().ms_copy_pages_most_pools())
+    if len(described) > most and max(*source, *destination) >= min(pages for *_, pages in described):
+        raise KernelError("copy_pages: a page lies outside the pools.")      # before the first launch
     for first in range(0, len(described), most):
         some = described[first : first + most]
         bases, page_bytes, calls, pages = zip(*some)
         call("ms_copy_pages", (ctypes.c_void_p * len(some))(*bases), (ctypes.c_int64 * len(some))(*page_bytes),
-             (ctypes.c_int32 * len(some))(*calls), (ctypes.c_int32 * len(some))(*pages), len(some), from_pages, to_pages, count, _stream())
+             (ctypes.c_int32 * len(some))(*calls), (ctypes.c_int32 * len(some))(*pages), len(some),
+             from_pages.buffer_info()[0], to_pages.buffer_info()[0], count, _stream())
 
 
 _EPILOGUE_BF16, _EPILOGUE_F32, _EPILOGUE_ADD_F32, _EPILOGUE_SILU_MUL = 0, 1, 2, 3

@@ -560,7 +560,8 @@ def test_refusals_of_the_gpu_side(ops):
         ("source of one copy", [pool], [0, 1], [1, 2]), ("source of one copy", [pool], [3], [3]), ("1 pages to 2", [pool], [0], [1, 2]),
         ("whole numbers", [pool], [0.0], [1]), ("whole numbers", [pool], [True], [2]), ("contiguous", [pool[:, :, ::2]], [0], [1]),
         ("calls>0", [torch.zeros(5, device=DEVICE)], [0], [1]), ("same memory", [pool, pool], [0], [1]),
-        ("same memory", [pool[1:], pool.view(1, 10, 8)], [0], [1]),
+        ("same memory", [pool[1:], pool.view(1, 10, 8)], [0], [1]), ("outside", [pool], [2**40], [1]),
+        ("outside", [torch.zeros(1, pages, 4, device=DEVICE) for pages in (5, 5, 5, 5, 3)], [4], [1]),
     ]:
         with pytest.raises(KernelError, match=match):
             ops.copy_pages(pools, source, destination)
