@@ -10,6 +10,8 @@ import array
 import contextlib
 import ctypes
 import dataclasses
+import functools
+import itertools
 import json
 import os
 import warnings
@@ -437,6 +439,7 @@ def can_share_prefix(head_dim: int, block_size: int) -> bool:
     return bool(load().ms_attention_shared_prefix_supported(head_dim, block_size))
 
 
+@functools.lru_cache(maxsize=512)
 def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, per_token: int, max_shared: int,
                          max_own: int, max_query: int, dtype: torch.dtype) -> tuple[int, int, int, int]:
     """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
@@ -485,6 +488,14 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
         return max(1, min(round(wanted), -(-keys // (128 if few else 256)), _DECODE_MAX_SPLITS))
 
     return tile, splits(room / parts, max_shared), own_tiles, splits((2 if few else 1) * units // own_parts, max_own)
+
+
+def _bound(name: str, given: int | None, most: int) -> int:
+    if given is None:
+        return most
+    if type(given) is not int or given < 0:
+        raise KernelError(f"attention_shared_prefix: {name} must be a whole number or None, not {given!r}.")
+    return max(1, min(given, most))
 
 
 def attention_shared_prefix(
@@ -556,13 +567,12 @@ def attention_shared_prefix(
     groups = group_start.numel() - 1
     shared_at = _address(shared_lens, "shared_lens", device, torch.int32, (groups,))
     longest = max_blocks * block_size
-    bounds = []
-    for name, given, most in (("max_sharing", max_sharing, groups), ("max_shared", max_shared, longest), ("max_own", max_own, longest), ("max_query", max_query, n)):
-        if given is not None and (type(given) is not int or given < 0):
-            raise KernelError(f"attention_shared_prefix: {name} must be a whole number or None, not {given!r}.")
-        bounds.append(max(1, most if given is None else min(given, most)))
+    max_sharing = _bound("max_sharing", max_sharing, groups)
+    max_shared, max_own = _bound("max_shared", max_shared, longest), _bound("max_own", max_own, longest)
+    max_query = _bound("max_query", max_query, n)
     per_token = heads // kv_heads
-    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(n * per_token, bounds[0], sequences, kv_heads, per_token, *bounds[1:], dtype)
+    tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(
+        n * per_token, max_sharing, sequences, kv_heads, per_token, max_shared, max_own, max_query, dtype)
     out = torch.empty_like(q)
     # of every part of a row's keys the outputs, then the maximum and the sum
     parts = n * heads * (shared_splits + own_splits)
@@ -586,16 +596,21 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
 
     if not isinstance(pools, (list, tuple)) or not pools:
         raise KernelError("copy_pages takes a list of at least one pool.")
-    described = []
-    for index, pool in enumerate(pools):
-        _check(pool, f"pools[{index}]")
-        if pool.ndim < 3 or pool.numel() == 0:
-            raise KernelError(f"copy_pages: pools[{index}] {tuple(pool.shape)} is not [calls>0, pages>0, ...].")
-        at = _address(pool, f"pools[{index}]", torch.cuda.current_device(), pool.dtype)
-        described.append((at, pool.stride(1) * pool.element_size(), pool.shape[0], pool.shape[1]))
-    ends = sorted((at, at + calls * pages * page_bytes) for at, page_bytes, calls, pages in described)
-    if any(after[0] < before[1] for before, after in zip(ends, ends[1:])):
-        raise KernelError("copy_pages: two pools lie in the same memory.")
+    device, described = None, []
+    for pool in pools:
+        _check(pool, "a pool")
+        if device is None:
+            device = torch.cuda.current_device()
+        at = _address(pool, "a pool", device, pool.dtype)
+        shape = pool.shape
+        if len(shape) < 3 or pool.numel() == 0:
+            raise KernelError(f"copy_pages: a pool {tuple(shape)} is not [calls>0, pages>0, ...].")
+        described.append((at, pool.stride(1) * pool.element_size(), shape[0], shape[1]))
+    end = 0
+    for at, page_bytes, calls, pages in sorted(described):
+        if at < end:
+            raise KernelError("copy_pages: two pools lie in the same memory.")
+        end = at + page_bytes * calls * pages
     count = len(source)
     if len(destination) != count:
         raise KernelError(f"copy_pages: {count} pages to {len(destination)} places.")
@@ -612,10 +627,9 @@ def copy_pages(pools: Sequence[torch.Tensor], source: Sequence[int], destination
         raise KernelError("copy_pages: a page lies outside the pools.")      # before the first launch
     for first in range(0, len(described), most):
         some = described[first : first + most]
-        bases, page_bytes, calls, pages = zip(*some)
-        call("ms_copy_pages", (ctypes.c_void_p * len(some))(*bases), (ctypes.c_int64 * len(some))(*page_bytes),
-             (ctypes.c_int32 * len(some))(*calls), (ctypes.c_int32 * len(some))(*pages), len(some),
-             from_pages.buffer_info()[0], to_pages.buffer_info()[0], count, _stream())
+        numbers = array.array("q", itertools.chain.from_iterable(some))
+        call("ms_copy_pages", numbers.buffer_info()[0], len(some), from_pages.buffer_info()[0], to_pages.buffer_info()[0],
+             count, _stream())
 
 
 _EPILOGUE_BF16, _EPILOGUE_F32, _EPILOGUE_ADD_F32, _EPILOGUE_SILU_MUL = 0, 1, 2, 3
@@ -1096,6 +1110,11 @@ def sample_rows(
     return out
 
 
+@functools.lru_cache(maxsize=512)
+def _verify_workspace_bytes(rows: int, requests: int, vocab: int) -> int:
+    return int(load().ms_verify_drafts_workspace_bytes(rows, requests, vocab))
+
+
 def verify_drafts(
     logits: torch.Tensor,
     row_start: torch.Tensor,
@@ -1145,11 +1164,11 @@ def verify_drafts(
         heat_at = _address(temperature, "temperature", device, torch.float32, (requests,))
         accept_at = _address(accept_uniform, "accept_uniform", device, torch.float32, drafts)
         draw_at = _address(draw_uniform, "draw_uniform", device, torch.float32, (requests,))
-    out = torch.empty(rows + requests, dtype=torch.int32, device=logits.device)
-    tokens, accepted = out.split((rows, requests))
-    size = int(load().ms_verify_drafts_workspace_bytes(rows, requests, vocab))
-    workspace = torch.empty(size, dtype=torch.uint8, device=logits.device)
-    out_at = out.data_ptr()
+    place = logits.device
+    tokens = torch.empty(rows, dtype=torch.int32, device=place)
+    accepted = torch.empty(requests, dtype=torch.int32, device=place)
+    size = _verify_workspace_bytes(rows, requests, vocab)
+    workspace = torch.empty(size, dtype=torch.uint8, device=place)
     call("ms_verify_drafts", logits_at, starts_at, tokens_at, probs_at if rows > requests else None, accept_at, draw_at, heat_at,
-         out_at, out_at + 4 * rows, workspace.data_ptr(), size, rows, requests, vocab, _stream())
+         tokens.data_ptr(), accepted.data_ptr(), workspace.data_ptr(), size, rows, requests, vocab, _stream())
     return tokens, accepted

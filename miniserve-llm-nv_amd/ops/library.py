@@ -34,7 +34,7 @@ _SIGNATURES: dict[str, list] = {
     "ms_attention_prefill_supported": [_I, _I],
     "ms_attention_shared_prefix": [_P] * 11 + [_I] * 8 + [_F] + [_I] * 5 + [_P],
     "ms_attention_shared_prefix_supported": [_I, _I],
-    "ms_copy_pages": [_P, _P, _P, _P, _I, _P, _P, _I, _P],
+    "ms_copy_pages": [_P, _I, _P, _P, _I, _P],
     "ms_copy_pages_most_pools": [],
     "ms_gemm_f32": [_P, _P, _P, _I, _I, _I, _I, _P],
     "ms_gemm_skinny": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
