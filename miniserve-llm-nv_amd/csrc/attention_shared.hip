@@ -26,9 +26,11 @@
 //
 // Measured on MI355X (bf16, head size 128, 8 kv heads, both kernels, recorded in a graph):
 //
-//   2 rows of 16 heads over 512 shared keys       8 us   start of two kernels and the chain
+//   2 rows of 16 heads over 512 shared keys,     10 us   one kernel a sequence whole: a unit's
+//     40 of their own                                     loads (283 KB at some 50 KB a us); in
+//                                                        parts 9, but 15 an eager call, not 11
+//   8 rows of 32 heads over 2,048                11 us   start of two kernels and the chain
 //                                                        table -> keys -> products of each
-//   8 rows of 32 heads over 2,048                11 us   the same
 //   45 rows of 32 heads, 7 groups of up to       39 us   161 MB in 33 us at a copy's rate; the
 //     5,000 and up to 700 keys of their own               sequences' own keys are most of it
 //   64 rows of 64 heads over 30,000             102 us   63 GFLOP: 0.62 PFLOP/s.  The products alone
@@ -39,6 +41,8 @@
 //
 // With every sequence reading its keys for itself the last three take 89 us (45 rows), 138 us
 // (16 rows with 5 tokens each over 4,096, here 19) and 632 us.
+#include <algorithm>
+
 #include "attention_columns.hpp"
 
 namespace {
@@ -719,6 +723,160 @@ __global__ __launch_bounds__(waves_of(ROWS) * ms::kWave) MS_WAVES_PER_EU(2, 2) v
   }
 }
 
+// Short sequences: a workgroup walks all keys of a sequence, the shared ones through the table of
+// the group's first and then its own, so that no parts are left and nothing is joined: one launch
+// instead of two, which is what an eager call of this size costs (times at ops.WHOLE_BYTES).
+// Workgroups: (kv head, tile of 16 rows, sequence).
+constexpr int kWholeWaves = 8;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kWholeWaves * ms::kWave) MS_WAVES_PER_EU(2, 2) void attention_shared_whole_kernel(
+    Sizes sizes, const int32_t* __restrict__ block_table, const int32_t* __restrict__ query_start,
+    const int32_t* __restrict__ context_lens, const int32_t* __restrict__ group_start,
+    const int32_t* __restrict__ shared_lens, const T* __restrict__ q, const T* __restrict__ key_pool,
+    const T* __restrict__ value_pool, T* __restrict__ out) {
+  using Op = Operand<T>;
+  constexpr int KS = Pair<T, D>::KS, CS = D / 16;
+  const Batch b{sizes, block_table, query_start, context_lens, group_start, shared_lens};
+  __shared__ __align__(16) float lds[direct_lds_bytes<D, kWholeWaves>() / sizeof(float)];
+  const int lane = threadIdx.x & 63, wave = ms::uniform(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int per_token = b.num_q_heads / b.num_kv_heads;
+  const int kv_head = blockIdx.x % b.num_kv_heads;
+  const int first_tile = blockIdx.x / b.num_kv_heads % b.own_tiles;
+  const int seq = blockIdx.x / b.num_kv_heads / b.own_tiles;
+  const int group = b.num_groups > 1 ? group_of_sequence(b, seq) : seq >= b.group_start[0] && seq < b.group_start[1] ? 0 : -1;
+  const int context = min(max(b.context_lens[seq], 0), b.most_keys);
+  const int first_token = b.query_start[seq], tokens = b.query_start[seq + 1] - first_token;
+  const int rows = tokens * per_token, pos_of_first = b.context_lens[seq] - tokens;
+  const int shared = group < 0 ? 0 : min(max(b.shared_lens[group], 0), b.most_keys);
+  const int from = min(shared, context), start = from / kTileKeys;
+  const int32_t* own_table = b.block_table + static_cast<int64_t>(seq) * b.max_blocks;
+  const int32_t* shared_table = group < 0 ? own_table : b.block_table + static_cast<int64_t>(b.group_start[group]) * b.max_blocks;
+  // pairs of tiles: those of the shared keys, then those of its own
+  const int shared_tiles = (shared + kTileKeys - 1) / kTileKeys, own_end = (context + kTileKeys - 1) / kTileKeys;
+  const int shared_pairs = (shared_tiles + 1) / 2;
+  const int pairs = shared_pairs + (context > from ? (own_end - start + 1) / 2 : 0);
+  const auto tile_of = [&](int pair) { return pair < shared_pairs ? 2 * pair : start + 2 * (pair - shared_pairs); };
+  const auto pages_of = [&](int pair) {
+    const bool of_group = pair < shared_pairs || context <= from;
+    return ms::find_pair_pages(min(tile_of(pair), (of_group ? shared_tiles : own_end) - 1), of_group ? shared_tiles : own_end,
+                               of_group ? shared_table : own_table, b.block_size);
+  };
+  const auto head_of = [&](int row, int& token) {
+    token = row / per_token;
+    return kv_head * per_token + row - token * per_token;
+  };
+  float* m_s = lds;                                      // [waves][16]
+  float* l_s = m_s + kWholeWaves * 16;                   // [waves][16]
+  float* o_s = l_s + kWholeWaves * 16;                   // [waves][16][D + 4]
+  constexpr int ROW = D + 4;
+
+  for (int tile = first_tile; tile * 16 < rows; tile += b.own_tiles) {
+    const int row = tile * 16 + r;
+    int token;
+    const int head = head_of(row, token);
+    const bool live = row < rows;
+    typename Op::V8 q_reg[KS];
+    const T* q_row = q + (static_cast<int64_t>(first_token + token) * b.num_q_heads + head) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = 32 * s + 8 * g;
+      q_reg[s] = live && d0 < D ? *reinterpret_cast<const typename Op::V8*>(q_row + d0) : Op::zero8();
+    }
+    RowState<D> st;
+#pragma unroll
+    for (int c = 0; c < CS; ++c) st.o[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+    st.run_max = -INFINITY;
+    st.run_sum = 0.f;
+    const int own_last = live ? min(context - 1, pos_of_first + token) : -1, shared_last = live ? shared - 1 : -1;
+    const auto use = [&](Pair<T, D>& pair, int p) {
+      const bool of_group = p < shared_pairs;
+      const int at = tile_of(p), first = of_group ? 0 : from, end = of_group ? shared : context;
+      if (at * kTileKeys < first || (at + 2) * kTileKeys > end) clear_outside<T, D>(pair, at, first, end, g);
+      consume<T, D>(st, pair, q_reg, at, first, of_group ? shared_last : own_last, b.scale * Op::kScale, g);
+    };
+    int p = wave;
+    if (p < pairs) {
+      // (a pair behind the end is looked up as the last one, and not loaded)
+      ms::PairPages pages = pages_of(p);
+      const auto load = [&](Pair<T, D>& pair, int of) {
+        load_pair<T, D>(pair, b, pages, key_pool, value_pool, kv_head, g, r);
+        pages = pages_of(of + kWholeWaves);
+      };
+      if constexpr (sizeof(T) == 2) {
+        Pair<T, D> ping, pong;
+        load(ping, p);
+        while (true) {
+          int next = p + kWholeWaves;
+          if (next < pairs) load(pong, next);
+          use(ping, p);
+          p = next;
+          if (p >= pairs) break;
+          next = p + kWholeWaves;
+          if (next < pairs) load(ping, next);
+          use(pong, p);
+          p = next;
+          if (p >= pairs) break;
+        }
+      } else {
+        for (; p < pairs; p += kWholeWaves) {
+          Pair<T, D> pair;
+          load(pair, p);
+          use(pair, p);
+        }
+      }
+    }
+    if (tile != first_tile) __syncthreads();      // what the tile before left in LDS is read
+    if (g == 0) {
+      m_s[wave * 16 + r] = st.run_max;
+      l_s[wave * 16 + r] = st.run_sum;
+    }
+#pragma unroll
+    for (int c = 0; c < CS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o_s[(wave * 16 + 4 * g + e) * ROW + 16 * c + r] = st.o[c][e];
+    __syncthreads();
+    constexpr int kAtOnce = kWholeWaves * ms::kWave / (D / 4);      // rows that the threads finish at once
+    const int d = 4 * (threadIdx.x % (D / 4));
+    for (int in_tile = threadIdx.x / (D / 4); in_tile < 16 && tile * 16 + in_tile < rows; in_tile += kAtOnce) {
+      if (threadIdx.x >= kAtOnce * (D / 4)) break;                  // threads that are left over
+      float mx = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kWholeWaves; ++v) mx = fmaxf(mx, m_s[v * 16 + in_tile]);
+      const float shift = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f;
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < kWholeWaves; ++v) {
+        const float factor = Op::weight(m_s[v * 16 + in_tile] - shift);      // 0 for a wave without keys
+        const floatx4 o = *reinterpret_cast<const floatx4*>(&o_s[(v * 16 + in_tile) * ROW + d]);
+        sum += factor * l_s[v * 16 + in_tile];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], factor, acc[e]);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      int token_of_row;
+      const int head_of_row = head_of(tile * 16 + in_tile, token_of_row);
+      T* to = out + (static_cast<int64_t>(first_token + token_of_row) * b.num_q_heads + head_of_row) * D + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] = ms::from_float<T>(acc[e] * inv);
+    }
+  }
+  // tokens before the first sequence and behind the last
+  if (first_tile == 0 && (seq == 0 || seq == b.num_seqs - 1)) {
+    const auto clear = [&](int token0, int token1) {
+      const int values = per_token * D;
+      for (int64_t i = threadIdx.x; i < static_cast<int64_t>(max(token1 - token0, 0)) * values; i += kWholeWaves * ms::kWave) {
+        const int64_t token = token0 + i / values;
+        out[(token * b.num_q_heads + kv_head * per_token) * D + i % values] = ms::from_float<T>(0.f);
+      }
+    };
+    if (seq == 0) clear(0, min(b.query_start[0], b.num_tokens));
+    if (seq == b.num_seqs - 1) clear(max(b.query_start[b.num_seqs], 0), b.num_tokens);
+  }
+}
+
 // Joins the parts of a row, a wave each.  A row that saw no key gives zeros, and so do the
 // rows of tokens before the first sequence and behind the last.
 constexpr int kJoinWaves = 4;
@@ -796,6 +954,15 @@ __global__ __launch_bounds__(kJoinWaves * ms::kWave) void attention_shared_join_
 template <typename T, int D>
 int launch(const Batch& b, const void* q, const void* key_pool, const void* value_pool, void* out, void* partial_o,
            void* partial_ml, hipStream_t stream) {
+  if (b.shared_splits == 0) {
+    hipLaunchKernelGGL((attention_shared_whole_kernel<T, D>),
+                       dim3(static_cast<unsigned>(b.num_seqs) * b.own_tiles * b.num_kv_heads), dim3(kWholeWaves * ms::kWave), 0,
+                       stream, static_cast<const Sizes&>(b), b.block_table, b.query_start, b.context_lens, b.group_start,
+                       b.shared_lens, static_cast<const T*>(q), static_cast<const T*>(key_pool),
+                       static_cast<const T*>(value_pool), static_cast<T*>(out));
+    MS_CHECK_LAUNCH("attention_shared_prefix (whole)");
+    return 0;
+  }
   const int units = b.num_kv_heads * b.shared_splits;
   const int64_t items = static_cast<int64_t>((units + kXcds - 1) / kXcds * kXcds) * b.shared_tiles +
                         static_cast<int64_t>(b.num_seqs) * b.own_tiles * b.own_splits * b.num_kv_heads;
@@ -853,7 +1020,8 @@ extern "C" int ms_attention_shared_prefix_supported(int head_dim, int block_size
 // [num_groups]; partial_o: float [num_tokens, num_q_heads, shared_splits + own_splits,
 // head_dim]; partial_ml: the same with 2 in head_dim's place.  rows_per_tile: 16, 32, 64
 // or 128 rows of a group a workgroup (32-bit storage: 16); own_tiles: workgroups that share
-// a sequence's tiles of 16 rows.
+// a sequence's tiles of 16 rows.  With 0 shared and 0 own splits every such workgroup walks all
+// keys of its sequence, and the workspaces are not used.
 extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, const void* value_pool,
                                           const void* block_table, const void* query_start, const void* context_lens,
                                           const void* group_start, const void* shared_lens, void* out, void* partial_o,
@@ -872,12 +1040,13 @@ extern "C" int ms_attention_shared_prefix(const void* q, const void* key_pool, c
              "attention_shared_prefix: tiles of %d rows", rows_per_tile);
   MS_REQUIRE(static_cast<int64_t>(num_kv_heads) * block_size * head_dim < (int64_t{1} << 31),
              "attention_shared_prefix: a page of %d kv heads x %d keys x %d is too large", num_kv_heads, block_size, head_dim);
-  MS_REQUIRE(shared_splits >= 1 && shared_splits <= kMaxSplits && own_splits >= 1 && own_splits <= kMaxSplits && own_tiles >= 1,
+  MS_REQUIRE(own_tiles >= 1 && ((shared_splits == 0 && own_splits == 0) ||
+                                (shared_splits >= 1 && shared_splits <= kMaxSplits && own_splits >= 1 && own_splits <= kMaxSplits)),
              "attention_shared_prefix: %d and %d splits are outside 1..%d", shared_splits, own_splits, kMaxSplits);
   MS_REQUIRE(dtype == MS_F32 || dtype == MS_BF16, "attention_shared_prefix: unknown dtype %d", dtype);
   const int64_t rows = static_cast<int64_t>(num_tokens) * (num_q_heads / num_kv_heads);
-  MS_REQUIRE(rows < (1LL << 31) - 4096 && rows / rows_per_tile + num_groups < (1LL << 24) / shared_splits &&
-                 static_cast<int64_t>(num_seqs) * own_tiles * own_splits < (1LL << 31) / num_kv_heads,
+  MS_REQUIRE(rows < (1LL << 31) - 4096 && rows / rows_per_tile + num_groups < (1LL << 24) / std::max(shared_splits, 1) &&
+                 static_cast<int64_t>(num_seqs) * own_tiles * std::max(own_splits, 1) < (1LL << 22) / num_kv_heads,
              "attention_shared_prefix: the batch is too large");
   Batch b;
   b.block_table = static_cast<const int32_t*>(block_table);

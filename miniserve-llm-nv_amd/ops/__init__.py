@@ -439,12 +439,21 @@ def can_share_prefix(head_dim: int, block_size: int) -> bool:
     return bool(load().ms_attention_shared_prefix_supported(head_dim, block_size))
 
 
+# Up to this many bytes of keys and values (a sequence's, of one kv head) and a workgroup a
+# compute unit at most, one kernel walks each sequence whole, without parts to join: a unit draws
+# some 50 KB a microsecond.  Measured on MI355X, 2 to 30 sequences, one kernel against parts and
+# their join: 65 KB 6.5 us against 9.2 recorded, 10.8 against 15.5 an eager call (the host's time);
+# 260 KB 11.2 against 9.6 and 10.8 against 15.5; 510 KB 17 against 10 and 15.7 against 15.5.
+WHOLE_BYTES = 300_000
+
+
 @functools.lru_cache(maxsize=512)
 def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, per_token: int, max_shared: int,
-                         max_own: int, max_query: int, dtype: torch.dtype) -> tuple[int, int, int, int]:
+                         max_own: int, max_query: int, dtype: torch.dtype, head_dim: int) -> tuple[int, int, int, int]:
     """How :func:`attention_shared_prefix` cuts its work: rows a tile of shared keys has,
     the parts those keys are cut into, the workgroups that share a sequence's tiles of 16
-    rows, and the parts that its own keys are cut into.  ``rows``: tokens times query heads
+    rows, and the parts that its own keys are cut into (0 and 0 parts: short sequences, each
+    walked whole).  ``rows``: tokens times query heads
     of a kv head; ``groups``: those that share keys.
 
     Fitted to a sweep on MI355X (head size 128, 1 to 64 sequences, 512 to 30,000 shared
@@ -466,6 +475,8 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
 
     own_tiles = -(-max_query * per_token // 16)
     own_parts = sequences * own_tiles * kv_heads
+    if own_parts <= units and (max_shared + max_own) * 2 * head_dim * dtype.itemsize <= WHOLE_BYTES:
+        return 16, 0, own_tiles, 0
     fewest_parts = -(-max_shared // 128)
     if dtype != torch.bfloat16 or rows <= 16 or tiles(16) * kv_heads * fewest_parts < 2 * units:
         tile = 16
@@ -515,7 +526,8 @@ def attention_shared_prefix(
     max_query: int | None = None,
 ) -> torch.Tensor:
     """Causal attention as :func:`attention` for sequences that share the front of their
-    cache, whose keys and values are read once a group instead of once a sequence.
+    cache, whose keys and values are read once a group instead of once a sequence (but for
+    short sequences, which the caches serve as well).
 
     ``q [N, heads, head_dim]``, pools and ``block_table [S, max_blocks]`` (int32) as there.
     Sequence ``s`` brings the tokens ``query_start[s] .. query_start[s + 1] - 1``, the last
@@ -572,14 +584,17 @@ def attention_shared_prefix(
     max_query = _bound("max_query", max_query, n)
     per_token = heads // kv_heads
     tile, shared_splits, own_tiles, own_splits = shared_prefix_launch(
-        n * per_token, max_sharing, sequences, kv_heads, per_token, max_shared, max_own, max_query, dtype)
+        n * per_token, max_sharing, sequences, kv_heads, per_token, max_shared, max_own, max_query, dtype, head_dim)
     out = torch.empty_like(q)
-    # of every part of a row's keys the outputs, then the maximum and the sum
-    parts = n * heads * (shared_splits + own_splits)
-    workspace = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
-    partial_o = workspace.data_ptr()
+    workspace = partial_o = partial_ml = None
+    if shared_splits > 0:
+        # of every part of a row's keys the outputs, then the maximum and the sum
+        parts = n * heads * (shared_splits + own_splits)
+        workspace = torch.empty(parts * (head_dim + 2), dtype=torch.float32, device=q.device)
+        partial_o = workspace.data_ptr()
+        partial_ml = partial_o + 4 * parts * head_dim
     call("ms_attention_shared_prefix", q_at, keys_at, values_at, table_at, starts_at, contexts_at, groups_at, shared_at,
-         out.data_ptr(), partial_o, partial_o + 4 * parts * head_dim, n, sequences, groups, heads, kv_heads, head_dim, block_size,
+         out.data_ptr(), partial_o, partial_ml, n, sequences, groups, heads, kv_heads, head_dim, block_size,
          max_blocks, float(scale), tile, shared_splits, own_tiles, own_splits, code, _stream())
     attention_calls["shared"] += 1
     return out

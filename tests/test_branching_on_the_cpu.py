@@ -411,16 +411,24 @@ def test_the_cut_of_the_work_stays_within_what_the_kernel_takes(monkeypatch):
     from miniserve_amd import ops
 
     monkeypatch.setattr(ops, "_decode_target", lambda: 512)
-    rng = random.Random(0)
+    ops.shared_prefix_launch.cache_clear()
+    rng, whole = random.Random(0), 0
     for _ in range(2000):
         sequences = rng.choice([1, 2, 7, 64, 500])
         groups = rng.randint(1, sequences)
         kv_heads, per_token, query = rng.choice([1, 2, 8]), rng.choice([1, 2, 3, 8, 24]), rng.choice([1, 2, 9, 70])
         longest = rng.choice([1, 100, 5000, 10**6])
         dtype = rng.choice([torch.float32, torch.bfloat16])
-        launch = ops.shared_prefix_launch(sequences * query * per_token, groups, sequences, kv_heads, per_token, longest, longest, query, dtype)
+        launch = ops.shared_prefix_launch(sequences * query * per_token, groups, sequences, kv_heads, per_token, longest, longest, query, dtype,
+                                          rng.choice([16, 64, 128]))
         tile, shared_splits, own_tiles, own_splits = launch
+        if shared_splits == own_splits == 0:       # a workgroup a sequence
+            whole += 1
+            assert longest <= 100 and tile == 16 and own_tiles >= 1
+            continue
         assert tile in ((16, 32, 64, 128) if dtype == torch.bfloat16 else (16,)) and 1 <= shared_splits <= 64 and 1 <= own_splits <= 64 and own_tiles >= 1
+    assert 100 < whole < 1900
+    ops.shared_prefix_launch.cache_clear()
 
 
 def test_the_plain_check_of_drafted_tokens_by_hand():

@@ -30,6 +30,17 @@ def ints(values):
 
 # ---- attention over a shared prefix ------------------------------------------------------
 
+@pytest.fixture(params=["parts", "whole"])
+def form(ops, request, monkeypatch):
+    """Keys cut into parts that a second kernel joins, or a workgroup a sequence (where that is
+    allowed at all): the rule decides by the keys' bytes, here every test runs both."""
+
+    monkeypatch.setattr(ops, "WHOLE_BYTES", 0 if request.param == "parts" else 10**15)
+    ops.shared_prefix_launch.cache_clear()
+    yield request.param
+    ops.shared_prefix_launch.cache_clear()
+
+
 def attention_case(dtype, heads, kv_heads, dim, page, groups, *, alone=(), seed=0, spare_rows=0, sharp=2.5):
     """``groups``: per group (shared keys, [(tokens, keys behind the shared ones), ...]);
     ``alone``: (tokens, context) of sequences behind the last group.  What no sequence holds
@@ -103,12 +114,14 @@ def check_attention(ops, case, out=None, **bounds):
     return out
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads", [(16, 8), (32, 8), (8, 1), (3, 3), (12, 4), (24, 1)])
 def test_one_group_of_single_tokens(ops, dtype, heads, kv_heads):
     check_attention(ops, attention_case(dtype, heads, kv_heads, 64, 16, [(160, [(1, 1), (1, 16), (1, 17), (1, 40), (1, 3)])]))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 112, 128])
 @pytest.mark.parametrize("page", [16, 32, 48])
@@ -116,6 +129,7 @@ def test_head_sizes_and_pages(ops, dtype, dim, page):
     check_attention(ops, attention_case(dtype, 8, 2, dim, page, [(2 * page, [(1, 5), (1, 33)]), (page, [(1, 1), (2, 2), (1, 70)])]))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shared", [1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 500])
 def test_shared_lengths_inside_pages_and_tiles(ops, dtype, shared):
@@ -123,6 +137,7 @@ def test_shared_lengths_inside_pages_and_tiles(ops, dtype, shared):
     check_attention(ops, attention_case(dtype, 8, 4, 64, 32, [(shared, [(1, 1), (1, 20), (1, 64)])], seed=shared))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_many_groups_of_all_sizes(ops, dtype):
     rng = random.Random(5)
@@ -130,6 +145,7 @@ def test_many_groups_of_all_sizes(ops, dtype):
     check_attention(ops, attention_case(dtype, 8, 2, 32, 16, groups, seed=3))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("rows", [16, 17, 33, 64, 65, 100, 128, 129, 200, 300])
 @pytest.mark.parametrize("dim,page", [(64, 16), (80, 48), (128, 16), (112, 32), (32, 64)])
 def test_rows_of_a_group_around_every_tile(ops, rows, dim, page):
@@ -140,11 +156,13 @@ def test_rows_of_a_group_around_every_tile(ops, rows, dim, page):
         check_attention(ops, attention_case(torch.bfloat16, heads, 1, dim, page, [(shared, members)], seed=rows + shared))
 
 
+@pytest.mark.usefixtures("form")
 def test_more_groups_than_a_wave_has_lanes(ops):
     groups = [(16 * (1 + g % 3), [(1, 1 + g % 7)] * (1 + g % 2)) for g in range(131)]
     check_attention(ops, attention_case(torch.bfloat16, 4, 2, 32, 16, groups, seed=4))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("tokens", [2, 5, 8, 33, 70])
 def test_drafted_tokens_see_each_other_causally(ops, dtype, tokens):
@@ -152,6 +170,7 @@ def test_drafted_tokens_see_each_other_causally(ops, dtype, tokens):
     check_attention(ops, attention_case(dtype, 8, 4, 64, 16, [(96, members)], seed=tokens))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_empty_groups_sequences_and_rows(ops, dtype):
     # a group without sequences, one that shares nothing, sequences that bring nothing, some in no group, a token whose
@@ -163,6 +182,7 @@ def test_empty_groups_sequences_and_rows(ops, dtype):
     assert bool(out[-4].any())
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_lengths_beyond_a_table_count_as_its_keys_and_rows_before_the_first_sequence_are_zero(ops, dtype):
     case = attention_case(dtype, 8, 4, 64, 16, [(64, [(1, 16), (1, 16)])], alone=[(1, 80)])
@@ -180,12 +200,14 @@ def test_lengths_beyond_a_table_count_as_its_keys_and_rows_before_the_first_sequ
     assert not bool(moved[:2].any()) and torch.equal(moved[2:], ops.attention_shared_prefix(**case))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_long_parts_are_split_and_joined(ops, dtype):
     check_attention(ops, attention_case(dtype, 4, 1, 64, 64, [(3000, [(1, 2100), (1, 1)])], seed=2))
     check_attention(ops, attention_case(dtype, 8, 2, 32, 16, [(1600, [(1, 1 + i) for i in range(40)])], seed=2))
 
 
+@pytest.mark.usefixtures("form")
 def test_bounds_that_are_too_small_or_missing_change_nothing_but_speed(ops):
     case = attention_case(torch.bfloat16, 8, 2, 64, 16, [(320, [(9, 40), (20, 333), (1, 1)]), (16, [(3, 80)])], seed=1)
     check_attention(ops, case)
@@ -194,6 +216,7 @@ def test_bounds_that_are_too_small_or_missing_change_nothing_but_speed(ops):
     check_attention(ops, case, max_shared=320, max_own=333, max_query=20)
 
 
+@pytest.mark.usefixtures("form")
 def test_scores_far_from_zero(ops):
     # sharp rows (one key carries everything) and scores of some hundreds: no overflow, no empty sum
     for scale in (30.0, 300.0):
@@ -201,6 +224,7 @@ def test_scores_far_from_zero(ops):
             check_attention(ops, attention_case(dtype, 8, 2, 64, 16, [(200, [(1, 30), (4, 9)])], sharp=scale, seed=int(scale)))
 
 
+@pytest.mark.usefixtures("form")
 def test_a_row_depends_only_on_its_sequence(ops):
     """Two calls on the same inputs give the same bits, and a poisoned group (NaN in all its
     keys) leaves the others alone."""
@@ -217,6 +241,7 @@ def test_a_row_depends_only_on_its_sequence(ops):
     assert torch.equal(first[:2], poisoned[:2]) and bool(poisoned[2:].isnan().all())
 
 
+@pytest.mark.usefixtures("form")
 def test_recorded_call_serves_other_lengths_and_groups(ops):
     """A recorded call replayed with other groups, lengths and queries in the same tensors,
     another recorded call and eager ones in between."""
@@ -264,6 +289,7 @@ def test_recorded_call_serves_other_lengths_and_groups(ops):
             check_attention(ops, case, out=call())
 
 
+@pytest.mark.usefixtures("form")
 def test_on_another_stream(ops):
     case = attention_case(torch.bfloat16, 8, 2, 64, 16, [(160, [(1, 20), (1, 40)])], seed=9)
     names = {k: v for k, v in case.items() if k not in ("q", "key_pool", "value_pool")}
@@ -276,6 +302,7 @@ def test_on_another_stream(ops):
     assert torch.equal(here, there)
 
 
+@pytest.mark.usefixtures("form")
 def test_pages_far_into_a_pool(ops):
     # offsets of elements past 2**31 and of bytes past 2**32
     page, dim, kv_heads = 16, 128, 8
