@@ -26,8 +26,8 @@
 //
 // Measured on MI355X (bf16, head size 128, 8 kv heads, both kernels, recorded in a graph):
 //
-//   2 rows of 16 heads over 512 shared keys,     10 us   one kernel a sequence whole: a unit's
-//     40 of their own                                     loads (283 KB at some 50 KB a us); in
+//   2 rows of 16 heads over 512 shared keys,     11 us   one kernel, a sequence whole: a unit's
+//     40 of their own                                     loads (283 KB at some 40 KB a us); in
 //                                                        parts 9, but 15 an eager call, not 11
 //   8 rows of 32 heads over 2,048                11 us   start of two kernels and the chain
 //                                                        table -> keys -> products of each

@@ -441,7 +441,7 @@ def can_share_prefix(head_dim: int, block_size: int) -> bool:
 
 # Up to this many bytes of keys and values (a sequence's, of one kv head) and a workgroup a
 # compute unit at most, one kernel walks each sequence whole, without parts to join: a unit draws
-# some 50 KB a microsecond.  Measured on MI355X, 2 to 30 sequences, one kernel against parts and
+# some 40 KB a microsecond.  Measured on MI355X, 2 to 30 sequences, one kernel against parts and
 # their join: 65 KB 6.5 us against 9.2 recorded, 10.8 against 15.5 an eager call (the host's time);
 # 260 KB 11.2 against 9.6 and 10.8 against 15.5; 510 KB 17 against 10 and 15.7 against 15.5.
 WHOLE_BYTES = 300_000
