@@ -193,19 +193,21 @@ class Sampler:
             accept += [self.draw_uniform(scratch) for _ in drafts]
             draw.append(self.draw_uniform(scratch))
             states.append(scratch.get_state())
-        # all numbers in one pinned buffer and one copy
-        sizes = [len(requests) + 1, drafted, drafted, len(requests), len(requests)]
+        # all numbers in one pinned buffer and one copy; where every request is greedy, without those for draws
+        greedy = all(state is None for state in states)
+        sizes = [len(requests) + 1, drafted] + ([] if greedy else [drafted, len(requests), len(requests)])
         host = torch.empty(sum(sizes), dtype=torch.float32, pin_memory=logits.is_cuda)
         starts = np.concatenate(([0], np.cumsum([count + 1 for count in counts])))
         numbers = [part.numpy() for part in host.split(sizes)]
         numbers[0].view(np.int32)[:] = starts
         numbers[1].view(np.int32)[:] = [token for _, _, drafts in requests for token in drafts]
-        numbers[2][:], numbers[3][:] = accept, draw
-        numbers[4][:] = [params.temperature for _, params, _ in requests]
+        if not greedy:
+            numbers[2][:], numbers[3][:] = accept, draw
+            numbers[4][:] = [params.temperature for _, params, _ in requests]
         sent = host.to(logits.device, non_blocking=True).split(sizes)
+        draws = {} if greedy else {"accept_uniform": sent[2], "draw_uniform": sent[3], "temperature": sent[4]}
         tokens, accepted = ops.verify_drafts(
-            logits.float().contiguous(), sent[0].view(torch.int32), sent[1].view(torch.int32), draft_probs=draft_probs,
-            accept_uniform=sent[2], draw_uniform=sent[3], temperature=sent[4],
+            logits.float().contiguous(), sent[0].view(torch.int32), sent[1].view(torch.int32), draft_probs=draft_probs, **draws,
         )
         chosen = torch.cat([tokens, accepted]).tolist()
         staged = []

@@ -454,6 +454,29 @@ def test_verify_drafts_greedy_and_sampled_requests_in_one_call(ops):
     assert (tokens.tolist(), accepted.tolist()) == want
 
 
+@pytest.mark.parametrize("vocab,drafts", [(1, [3, 0, 2]), (130, [0, 1] * 300), (5003, [0, 40, 7, 1, 5]), (151936, [2, 4])])
+def test_verify_drafts_without_temperatures(ops, vocab, drafts):
+    """All requests greedy, said by leaving the temperatures out: as with temperatures of 0."""
+
+    case = draft_case(drafts, vocab, temperature=0.0, agree=0.02, seed=vocab)
+    if len(drafts) == 5:
+        case["logits"][int(case["row_start"][1]) + 3, 17] = float("inf")
+    taken = check_verify(ops, case)
+    sent = [case[name].to(DEVICE) for name in ("logits", "row_start", "draft_tokens")]
+    tokens, accepted = ops.verify_drafts(*sent)
+    assert accepted.tolist() == taken and max(taken) > 0
+    assert torch.equal(tokens, run_verify(ops, case)[0])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        again = ops.verify_drafts(*sent)
+    for _ in range(3):
+        again[0].fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again[0], tokens) and torch.equal(again[1], accepted)
+
+
 def test_verify_drafts_all_taken_none_taken_and_only_next_tokens(ops):
     case = draft_case([4, 4], 999, seed=5)
     case["accept_uniform"][:] = 0.0
