@@ -21,9 +21,9 @@
 // are taken, by every workgroup of the request for itself, and the masses of a chunk of w and
 // p at the row where they end; (3) the draw: the chunk by the chunks' masses, then the token.
 //
-// (1) reads every logit once, and with some 25 64-bit instructions an element those and the
-// read take about as long: 576 rows of 151,936, 350 MB, 76 us = 4.6 TB/s on MI355X (a large
-// copy: 4.9); with 64 requests of 8 drafts (2), (2a) and (3) take 33 us more.  One request of 4
+// (1) reads every logit once, and with some 22 64-bit instructions an element those and the
+// read take about as long: 576 rows of 151,936, 350 MB, 64 to 76 us = 4.6 to 5.5 TB/s on
+// MI355X (a large copy: 4.9); with 64 requests of 8 drafts (2), (2a) and (3) take 33 us more.  One request of 4
 // drafts takes 6 + 6 + 6 us, each the chain of its loads and sums over a workgroup.  (With the
 // draw in (2), by the request's last workgroup, each has to make its masses visible to the
 // other dies' caches: 110 us instead of 28 for (2) and (3) of 64 requests, 13 as before for one.)
@@ -37,11 +37,14 @@ namespace {
 constexpr int kRowChunk = 2048, kChunk = 4096;
 constexpr int kRowThreads = 256, kChooseThreads = 512, kDrawThreads = kChunk / 4;
 
-// 2^f on -1/2 .. 1/2, lowest power first: the polynomial of degree nine whose largest relative
-// error there is least (found by exchange of its extrema: 1.3e-14).  It travels with a kernel's
-// arguments, so that its coefficients lie in scalar registers: as literals the compiler copies
-// each into vector registers before every use (39 instructions an element instead of 25).
-constexpr int kDegree = 9;
+// 2^f on -1/2 .. 1/2, lowest power first: the polynomials of degree seven and nine whose largest
+// relative error there is least (found by exchange of its extrema: 4.0e-11 and 1.3e-14).  They
+// travel with a kernel's arguments, so that the coefficients lie in scalar registers: as literals
+// the compiler copies each into vector registers before every use (39 instructions an element
+// instead of 25).  The shorter one serves Z, the sum over all tokens of all rows (76 us for 576
+// rows, with the longer one 89): it moves a border by 4e-11 of itself at most, past one uniform
+// number in some 10^10.
+constexpr int kDegree = 9, kSumDegree = 7;
 constexpr double kPowerOfTwo[kDegree + 1] = {
     1.00000000000001266e+00,
     6.93147180559871012e-01,
@@ -54,9 +57,19 @@ constexpr double kPowerOfTwo[kDegree + 1] = {
     1.32594056112041923e-06,
     1.01503372609764174e-07,
 };
+constexpr double kSumPowerOfTwo[kSumDegree + 1] = {
+    9.99999999961681983e-01,
+    6.93147180728445564e-01,
+    2.40226511981572074e-01,
+    5.55041035345320847e-02,
+    9.61802725371136973e-03,
+    1.33339225590775260e-03,
+    1.54692911308010617e-04,
+    1.52019226419755618e-05,
+};
 
 struct Batch {
-  double power[kDegree + 1];
+  double power[kDegree + 1], sum_power[kSumDegree + 1];
   const float* __restrict__ logits;
   const int32_t* __restrict__ row_start;
   const int32_t* __restrict__ draft_tokens;
@@ -109,16 +122,17 @@ __device__ __forceinline__ float temperature_of(const Batch& b, int request) {
 // instructions, so that k is had by adding 3 * 2^51, which leaves it in the sum's low bits, and
 // 2^k by adding k to the exponent's bits (conversions and scalings run at a quarter of an
 // addition's rate).  Below 2^-1000 the result is 2^-1000 at most and not 0.
-__device__ __forceinline__ double pow2_floored(const Batch& b, double x) {
+template <int DEGREE>
+__device__ __forceinline__ double pow2_floored(const double (&power)[DEGREE + 1], double x) {
   x = fmax(x, -1001.0);
   const double shifted = x + 6755399441055744.0;
   const double f = x - (shifted - 6755399441055744.0);
-  double r = b.power[kDegree];
+  double r = power[DEGREE];
 #pragma unroll
-  for (int n = kDegree - 1; n >= 0; --n) r = fma(r, f, b.power[n]);
+  for (int n = DEGREE - 1; n >= 0; --n) r = fma(r, f, power[n]);
   return __hiloint2double(__double2hiint(r) + (__double2loint(shifted) << 20), __double2loint(r));
 }
-__device__ __forceinline__ double pow2(const Batch& b, double x) { return x < -1000.0 ? 0.0 : pow2_floored(b, x); }
+__device__ __forceinline__ double pow2(const Batch& b, double x) { return x < -1000.0 ? 0.0 : pow2_floored<kDegree>(b.power, x); }
 
 // e^{(l - max) / temperature} = 2^{(l - max) * rate}
 __device__ __forceinline__ double rate_of(float temperature) { return 1.4426950408889634074 / static_cast<double>(temperature); }
@@ -213,20 +227,20 @@ __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(Batch b, RowPa
   double sum = 0.0;
   int place = 0x7fffffff;
   if (temperature > 0.f) {
-    const double rate = rate_of(temperature);
+    const double rate = rate_of(temperature), offset = -static_cast<double>(best) * rate;
     // (a sum that holds a mass of 1 does not see one of 2^-1000)
     if (q.whole) {
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += pow2_floored(b, exponent_of(q.value[j][i], best, rate));
+        for (int i = 0; i < 4; ++i) sum += pow2_floored<kSumDegree>(b.sum_power, fma(static_cast<double>(q.value[j][i]), rate, offset));
     } else {
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = q.first[j] + i;
-          const double mass = pow2_floored(b, exponent_of(q.value[j][i], best, rate));
+          const double mass = pow2_floored<kSumDegree>(b.sum_power, fma(static_cast<double>(q.value[j][i]), rate, offset));
           sum += e >= 0 && e < b.vocab ? mass : 0.0;
         }
     }
@@ -566,6 +580,7 @@ extern "C" int ms_verify_drafts(const void* logits, const void* row_start, const
   MS_REQUIRE(workspace_bytes >= ms_verify_drafts_workspace_bytes(rows, requests, vocab), "verify_drafts: workspace too small");
   Batch b;
   for (int n = 0; n <= kDegree; ++n) b.power[n] = kPowerOfTwo[n];
+  for (int n = 0; n <= kSumDegree; ++n) b.sum_power[n] = kSumPowerOfTwo[n];
   b.logits = static_cast<const float*>(logits);
   b.row_start = static_cast<const int32_t*>(row_start);
   b.draft_tokens = static_cast<const int32_t*>(draft_tokens);
