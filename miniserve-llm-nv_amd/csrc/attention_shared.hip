@@ -9,7 +9,8 @@
 //   out = sum_c e^{m_c - M} O_c / sum_c e^{m_c - M} l_c,   M = max_c m_c
 //
 // The parts here are splits of the group's shared keys and splits of the sequence's own
-// keys behind them.  One kernel makes the (m, l, O) of all parts, a second joins them.
+// keys behind them.  One kernel makes the (m, l, O) of all parts, a second joins them; sequences
+// that are short enough are walked whole, by a kernel of their own that leaves no parts.
 //
 // A workgroup takes a tile of rows of one kv head (rows of the whole group for
 // shared keys, of one sequence for its own) and a range of keys, dealt out to the waves in
