@@ -112,3 +112,62 @@ def test_sampled_drafts_on_the_device_take_the_plain_choice(model_folders):
     finally:
         ops.verify_drafts = kernel
     assert [(s.token_ids, s.accepted) for s in got] == [(s.token_ids, s.accepted) for s in want]
+
+
+def test_branches_in_steps_that_are_launched_ahead(model_folders, monkeypatch):
+    """Four branches decode in recorded steps whose numbers are prepared, and which are launched,
+    before the host has read the tokens of the step before; one such step is thrown away, and
+    a branch is cut and another forked between them.  Greedy tokens, every row of logits
+    against the plain implementation."""
+
+    from miniserve_amd import ops
+    from miniserve_amd.engine import StepEntry, batch
+
+    monkeypatch.setattr(batch, "SHARED_FRONT_KEYS", 256)
+    folder, block_size = model_folders["a"]
+    config, weights = read_config(folder), read_weights(folder)
+    runner = make_runner(folder, block_size, "bfloat16", recorded=True)
+    branches = branching_run.Branches(runner, config["vocab_size"], seed=77)
+    branches.admit("p")
+    branches.step(p=290)
+    branches.fork("p", "a", "b", "c")
+    names = ["p", "a", "b", "c"]
+
+    def keep(logits):
+        for name, row in zip(names, logits.float().cpu()):
+            branches.rows.append((list(branches.tokens[name]), row))
+        return ops.sample_rows(logits.float().contiguous())
+
+    def eager_tokens():
+        tokens = {}
+        for i, name in enumerate(names):
+            tokens[name] = (17 * i + len(branches.tokens[name])) % config["vocab_size"]
+            branches.tokens[name].append(tokens[name])
+        return [StepEntry(name, (tokens[name],), (0,)) for name in names]
+
+    chained = 0
+    for part in range(3):
+        tokens = keep(runner.step(eager_tokens()))
+        for turn in range(4):
+            prepared = runner.prepare_decode(names)
+            assert prepared is not None
+            runner.launch_chained(prepared, tokens)
+            chosen = tokens.tolist()
+            if turn == 3:
+                runner.discard(prepared)
+                break
+            for name, token in zip(names, chosen):
+                branches.tokens[name].append(token)
+            tokens = keep(runner.step([StepEntry(name, (token,), (0,)) for name, token in zip(names, chosen)], prepared))
+            chained += 1
+        runner.cache.assert_invariants()
+        if part == 0:
+            branches.truncate("b", len(branches.tokens["b"]) - 2)
+        if part == 1:
+            branches.release("c")
+            branches.fork("a", "d", "e")
+            names = ["p", "b", "a", "d", "e"]    # two runs now
+    keys = [key for key in runner._decode_graphs if len(key) == 3]
+    assert runner.chained_steps == chained + 3 and keys and {key[2][0] for key in keys} == {1, 2}
+    worst, allowed = branches.worst(weights, config, "bfloat16")
+    assert worst <= allowed, f"{worst:.3e} > {allowed:.3e}"
