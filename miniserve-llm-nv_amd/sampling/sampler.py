@@ -175,6 +175,10 @@ class Sampler:
                 raise ValueError(f"request {request_id!r}: drafted tokens are compared with whole distributions, without top-k and top-p.")
             if any(type(token) is not int or token < 0 for token in drafts):
                 raise ValueError(f"request {request_id!r}: drafted tokens must be non-negative integers.")
+            if logits.ndim == 2 and any(token >= logits.shape[1] for token in drafts):
+                raise ValueError(f"request {request_id!r}: a drafted token is outside the vocabulary of {logits.shape[1]}.")
+        if len({request_id for request_id, _, _ in requests}) != len(requests):
+            raise ValueError("a request is named twice; its second turn draws behind its first one's commit.")
         counts = [len(drafts) for _, _, drafts in requests]
         rows, drafted = sum(counts) + len(requests), sum(counts)
         if not requests or logits.ndim != 2 or logits.shape[0] != rows:

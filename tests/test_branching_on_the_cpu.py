@@ -384,7 +384,8 @@ def test_drafted_tokens_take_numbers_from_the_requests_own_stream(monkeypatch):
     bad[3, 7] = float("nan")       # behind the draft that is not taken: never reached
     assert sampler.stage_drafts(bad, requests)[0].token_ids == staged[0].token_ids
     for wrong, match in (([("s", SamplingParams(temperature=1.0, top_p=0.9), [1])], "top-p"), ([("s", SamplingParams(temperature=1.0, top_k=4), [1])], "top-k"),
-                         ([("s", SamplingParams(), [-1])], "non-negative"), ([("s", SamplingParams(), [1, 2])], "rows of logits"), ([], "rows of logits")):
+                         ([("s", SamplingParams(), [-1])], "non-negative"), ([("s", SamplingParams(), [logits.shape[1]])], "vocabulary"),
+                         ([("s", SamplingParams(), []), ("s", SamplingParams(), [])], "named twice"), ([("s", SamplingParams(), [1, 2])], "rows of logits"), ([], "rows of logits")):
         with pytest.raises(ValueError, match=match):
             sampler.stage_drafts(logits[:2], wrong)
 
