@@ -118,29 +118,33 @@ __device__ __forceinline__ float temperature_of(const Batch& b, int request) {
   return b.temperature != nullptr ? b.temperature[request] : 0.f;
 }
 
-// 2^x in 64 bits for x <= 0: 2^k 2^f with k the nearest whole number.  (1) is bound by these
-// instructions, so that k is had by adding 3 * 2^51, which leaves it in the sum's low bits, and
-// 2^k by adding k to the exponent's bits (conversions and scalings run at a quarter of an
-// addition's rate).  Below 2^-1000 the result is 2^-1000 at most and not 0.
+// e^{(l - max) / T} = 2^{d rate}, d = l - max, rate = log2(e) / T
+__device__ __forceinline__ double rate_of(float temperature) { return 1.4426950408889634074 / static_cast<double>(temperature); }
+
+// 2^{d rate} in 64 bits for d rate from -1001 to 0: 2^k 2^f with k the nearest whole number.  (1) is
+// bound by these instructions, so that k is had by adding 3 * 2^51, which leaves it in the sum's low
+// bits, and 2^k by adding k to the exponent's bits (conversions and scalings run at a quarter of an
+// addition's rate).  The product is made inside the two multiply-adds and never rounded by itself.
+// d has to be the logits' difference: with l and max multiplied each for itself, the rounding of
+// max * rate, up to |max| rate 2^-53, is left over at the maximum, and at T = 10^-15 or logits
+// of 10^16 that is more than the mass itself.
 template <int DEGREE>
-__device__ __forceinline__ double pow2_floored(const double (&power)[DEGREE + 1], double x) {
-  x = fmax(x, -1001.0);
-  const double shifted = x + 6755399441055744.0;
-  const double f = x - (shifted - 6755399441055744.0);
+__device__ __forceinline__ double pow2_scaled(const double (&power)[DEGREE + 1], double d, double rate) {
+  const double shifted = fma(d, rate, 6755399441055744.0);
+  const double f = fma(d, rate, -(shifted - 6755399441055744.0));
   double r = power[DEGREE];
 #pragma unroll
   for (int n = DEGREE - 1; n >= 0; --n) r = fma(r, f, power[n]);
   return __hiloint2double(__double2hiint(r) + (__double2loint(shifted) << 20), __double2loint(r));
 }
-__device__ __forceinline__ double pow2(const Batch& b, double x) { return x < -1000.0 ? 0.0 : pow2_floored<kDegree>(b.power, x); }
 
-// e^{(l - max) / temperature} = 2^{(l - max) * rate}
-__device__ __forceinline__ double rate_of(float temperature) { return 1.4426950408889634074 / static_cast<double>(temperature); }
-__device__ __forceinline__ double exponent_of(float logit, float max, double rate) {
-  return (static_cast<double>(logit) - static_cast<double>(max)) * rate;
-}
+// The least d of pow2_scaled: -1001 / rate.
+__device__ __forceinline__ double floor_of(float temperature) { return -1001.0 * 0.69314718055994530942 * static_cast<double>(temperature); }
+
 __device__ __forceinline__ double mass_of(const Batch& b, float logit, float max, double rate) {
-  return pow2(b, exponent_of(logit, max, rate));
+  const double d = static_cast<double>(logit) - static_cast<double>(max);
+  const double mass = pow2_scaled<kDegree>(b.power, d, rate);
+  return d * rate < -1000.0 ? 0.0 : mass;
 }
 
 __device__ __forceinline__ bool not_finite(float v) { return __builtin_isfpclass(v, 0x3 | 0x4 | 0x200); }      // NaN, -inf, +inf
@@ -227,21 +231,24 @@ __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(Batch b, RowPa
   double sum = 0.0;
   int place = 0x7fffffff;
   if (temperature > 0.f) {
-    const double rate = rate_of(temperature), offset = -static_cast<double>(best) * rate;
-    // (a sum that holds a mass of 1 does not see one of 2^-1000)
+    const double rate = rate_of(temperature), least = floor_of(temperature), top = best;
+    // what lies below the least is taken as 2^-1001: a sum that holds a mass of 1 does not see it
+    const auto mass = [&](float logit) {
+      return pow2_scaled<kSumDegree>(b.sum_power, fmax(static_cast<double>(logit) - top, least), rate);
+    };
     if (q.whole) {
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += pow2_floored<kSumDegree>(b.sum_power, fma(static_cast<double>(q.value[j][i]), rate, offset));
+        for (int i = 0; i < 4; ++i) sum += mass(q.value[j][i]);
     } else {
 #pragma unroll
       for (int j = 0; j < kQuads; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = q.first[j] + i;
-          const double mass = pow2_floored<kSumDegree>(b.sum_power, fma(static_cast<double>(q.value[j][i]), rate, offset));
-          sum += e >= 0 && e < b.vocab ? mass : 0.0;
+          const double here = mass(q.value[j][i]);
+          sum += e >= 0 && e < b.vocab ? here : 0.0;
         }
     }
     sum = lanes_sum<ms::kWave>(sum);
