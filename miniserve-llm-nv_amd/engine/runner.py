@@ -79,7 +79,8 @@ class DecodeGraph:
 
     ``shared``: of a recording for steps with neighbouring rows of forked requests, the most
     runs of them and the most keys that a row does not share; where the runs lie and how
-    many keys they share is among the step's numbers.
+    many keys they share is among the step's numbers, for each group of pages without a window
+    (layers with one read no common pages, and pages of another size have other runs).
     """
 
     def __init__(self, runner: "ModelRunner", batch: int, bound: int, shared: tuple[int, int] | None = None) -> None:
@@ -90,6 +91,7 @@ class DecodeGraph:
         # and not at some later collection of cycles
         self._runner = weakref.ref(runner)
         groups = len(runner.cache.layout.groups)
+        self._sharing = [shared is not None and group.window is None for group in runner.cache.layout.groups]
         widths = tuple(-(-bound // size) for size in runner.cache.block_sizes)     # per group: pages of a row at the bound
         # the parts' own tables, from what every replay shares: one token a row
         host_batch = HostBatch((1,) * batch, tuple(range(batch + 1)), None, batch, recorded=True)
@@ -100,7 +102,7 @@ class DecodeGraph:
         sizes += [(f"part:{name}", values.size) for name, values in part_tables.items()]
         for group in range(groups):
             sizes += [(f"slots{group}", batch), (f"table{group}", batch * widths[group])]
-            if shared is not None:
+            if self._sharing[group]:
                 sizes += [(f"front_start{group}", 2 * shared[0] + 1), (f"front_lens{group}", 2 * shared[0])]
         # for a step launched behind the sampling of the step before: which of that step's rows each row continues
         sizes += [("token_rows", batch)]
@@ -132,8 +134,8 @@ class DecodeGraph:
             state_slots=view("state_slots"),
             groups=[
                 GroupStepView(block_table=view(f"table{g}").view(batch, widths[g]), slot_mapping=view(f"slots{g}"),
-                              shared=None if shared is None else SharedFronts(
-                                  view(f"front_start{g}"), view(f"front_lens{g}"), shared[0], bound, shared[1], 1))
+                              shared=SharedFronts(view(f"front_start{g}"), view(f"front_lens{g}"), shared[0], bound, shared[1], 1)
+                              if self._sharing[g] else None)
                 for g in range(groups)
             ],
             # what holds for every replay: one token a row.  Launch decisions inside the
@@ -185,7 +187,7 @@ class DecodeGraph:
         put("logit_rows", range(batch))
         forks, contexts = [meta.fork for meta in metas], [meta.after for meta in metas]
         for group in range(len(runner.cache.layout.groups)):
-            if self.shared is not None:
+            if self._sharing[group]:
                 # groups that are not there, and rows in none, share nothing
                 fronts = shared_fronts(forks, contexts, group, runner.cache.block_sizes[group])
                 starts, lens = (fronts.starts, fronts.lens) if fronts is not None else ([0], [])
