@@ -83,6 +83,7 @@ class StepItem:
     request_id: str
     start: int        # first new position = tokens already committed
     end: int          # length after the step
+    keep: int | None = None      # the least length that the request may be cut to behind the step (None: end)
 
 
 @dataclass(eq=False)
@@ -105,6 +106,7 @@ class SequenceStepMeta:
     slot_mappings: list[tuple[int, ...]]    # per group, one slot per new token
     new_pages: list[list[int]]              # per group
     fork: Fork | None = None                # whom the request shares its first pages with
+    keep: int | None = None                 # the least length that it may be cut to afterwards (None: after)
 
 
 @dataclass
@@ -125,6 +127,7 @@ class _Live:
     pending: bool = False
     fork: Fork | None = None
     branched: bool = False      # took part in a fork, so that others may hold pages of its tables
+    kept: bool = False          # holds pages that a window has passed, for a cut
 
 
 class CacheManager:
@@ -345,7 +348,8 @@ class CacheManager:
                 forked.extend(pages[index : index + 1])
                 tables.append(forked)
             slot = self._free_slots.pop()
-            self._live[child] = _Live(child, slot, committed=live.committed, tables=tables, fork=fork, branched=True)
+            self._live[child] = _Live(child, slot, committed=live.committed, tables=tables, fork=fork, branched=True,
+                                      kept=live.kept)
             for tensor in self.state_tensors:
                 tensor[slot].copy_(tensor[live.state_slot])
             slots.append(slot)
@@ -356,12 +360,14 @@ class CacheManager:
         not taken, say) and give their pages back.  A last page that others hold too is
         replaced by a copy first, since the next step writes into it.  Refused for a model
         with state, which cannot be taken back, and where a window's pages that were given
-        back would be needed again.  When a page for a copy is missing nothing has changed."""
+        back would be needed again: below what the last step kept (``StepItem.keep``).  When a
+        page for a copy is missing nothing has changed."""
 
         live = self._settled(request_id)
         if type(length) is not int or not 0 <= length <= live.committed:
             raise CacheError(f"request {request_id!r} holds {live.committed} tokens, it cannot be cut to {length!r}.")
         if length == live.committed:
+            self._give_back_passed_pages(live)
             return
         if self.layout.states:
             raise CacheError("a model with per-request state cannot take tokens back.")
@@ -389,6 +395,7 @@ class CacheManager:
         live.committed = length
         if live.fork is not None and any(length < count * size for count, size in zip(live.fork.pages, self.block_sizes)):
             live.fork = None
+        self._give_back_passed_pages(live)
 
     def compact(self) -> int:
         """Move pages so that those in use are the first of their pools; returns how many
@@ -433,13 +440,19 @@ class CacheManager:
                 )
             if item.end <= item.start or item.end > self.max_model_len:
                 raise CacheError(f"request {item.request_id!r}: the step ends at {item.end} (limit {self.max_model_len}).")
+            if item.keep is not None and not item.start <= item.keep <= item.end:
+                raise CacheError(f"request {item.request_id!r}: a step from {item.start} to {item.end} cannot keep {item.keep}.")
+        for item in items:
+            live = self._live[item.request_id]
+            if live.kept:       # a request that goes on is not cut any more
+                self._give_back_passed_pages(live)
         reservation = StepReservation(self._next_step_id)
         self._next_step_id += 1
         taken: list[tuple[int, list[int]]] = []
         try:
             for item in items:
                 live = self._live[item.request_id]
-                meta = SequenceStepMeta(item.request_id, live.state_slot, item.start, item.end, [], [], [], live.fork)
+                meta = SequenceStepMeta(item.request_id, live.state_slot, item.start, item.end, [], [], [], live.fork, item.keep)
                 for index, (allocator, table) in enumerate(zip(self.allocators, live.tables)):
                     missing = table.pages_for(item.end) - len(table.pages)
                     new_pages = allocator.allocate(max(missing, 0))
@@ -499,7 +512,7 @@ class CacheManager:
                 table.extend(pages)
             live.committed = meta.after
             live.pending = False
-            self._give_back_passed_pages(live)
+            self._give_back_passed_pages(live, meta.keep)
 
     def abort_step(self, reservation: StepReservation) -> None:
         """Gives exactly the step's new pages back and restores the state of its
@@ -521,14 +534,18 @@ class CacheManager:
         reservation.closed = True
         self._open = None
 
-    def _give_back_passed_pages(self, live: _Live) -> None:
+    def _give_back_passed_pages(self, live: _Live, keep: int | None = None) -> None:
         """With ``n`` tokens committed the next query stands at ``n`` or later and
-        reads keys ``>= n - window + 1``; pages wholly below that go back."""
+        reads keys ``>= n - window + 1``; pages wholly below that go back.  ``keep``: where the next
+        query may stand yet, when tokens of the last step turn out to be forgotten; the pages
+        from there on are given back by the cut, or by the request's next step."""
 
+        length = live.committed if keep is None else keep
+        live.kept = length < live.committed
         for group, allocator, table in zip(self.layout.groups, self.allocators, live.tables):
             if group.window is None:
                 continue
-            pages = table.give_back_before(live.committed - group.window + 1)
+            pages = table.give_back_before(length - group.window + 1)
             if pages:
                 allocator.release(pages)
 

@@ -482,7 +482,9 @@ class ModelRunner:
     @torch.inference_mode()
     def truncate(self, request_id: str, length: int) -> None:
         """Forget the request's tokens behind the first ``length``: drafted tokens that were
-        run by a step and not taken (``Sampler.stage_drafts``)."""
+        run by a step and not taken (``Sampler.stage_drafts``).  A model with a window holds
+        what that takes for the tokens behind the first place whose logits the last step
+        wanted, until the request's next step."""
 
         self.cache.truncate(request_id, length)
 
@@ -583,10 +585,15 @@ class ModelRunner:
             self.release(request_id)
 
     def _open_step(self, entries: Sequence[StepEntry]):
+        """An entry that wants logits before its last place brings drafted tokens, it may be: what
+        stands behind the first wanted place may have to be forgotten (:meth:`truncate`)."""
+
         items = []
         for entry in entries:
             start = self.cache.committed_tokens(entry.request_id)
-            items.append(StepItem(entry.request_id, start, start + len(entry.token_ids)))
+            count = len(entry.token_ids)
+            keep = start + min(entry.want) + 1 if count > 1 and entry.want else None
+            items.append(StepItem(entry.request_id, start, start + count, keep))
         return self.cache.prepare_step(items)
 
     @torch.inference_mode()

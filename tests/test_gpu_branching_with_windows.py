@@ -24,3 +24,13 @@ def test_runs_of_neighbours_differ_between_groups_of_pages(recorded, model_folde
     assert ops.attention_calls["shared"] > before
     if recorded:
         assert {key[2] for key in runner._decode_graphs if len(key) == 3} == {(1, 256)}
+
+
+@pytest.mark.parametrize("recorded", [False, True], ids=["eager", "recorded"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_drafts_in_a_model_with_a_window(dtype, recorded, model_folders):
+    folder, block_size = model_folders["c"]
+    runner = windowed.make_runner(folder, block_size, dtype, device="cuda:0", recorded=recorded)
+    branches = windowed.rounds_of_drafts(runner, read_config(folder)["vocab_size"], rounds=25, seed=31)
+    found, allowed = windowed.worst(branches, folder, dtype)
+    assert found <= allowed, f"{found:.3e} > {allowed:.3e}"

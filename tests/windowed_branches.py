@@ -74,3 +74,30 @@ def five_branches_and_three_pairs(runner, vocab: int) -> branching_run.Branches:
     for _ in range(3):
         branches.step(**{name: 1 for name in names})
     return branches
+
+
+def rounds_of_drafts(runner, vocab: int, *, rounds: int, seed: int) -> branching_run.Branches:
+    """Two requests that bring drafted tokens and lose some, or all, of them again, over several
+    windows; a branch that is made before its parent's drafts are decided goes on beside it."""
+
+    import random
+
+    rng = random.Random(seed)
+    branches = branching_run.Branches(runner, vocab, seed=seed)
+    for name, prompt in (("p", 30), ("q", 61)):
+        branches.admit(name)
+        branches.step(**{name: prompt})
+    for turn in range(rounds):
+        counts = {name: 1 + rng.randint(0, 12) for name in branches.tokens}
+        branches.step(**counts)
+        if turn == rounds // 2:
+            branches.fork("p", "x")
+            counts["x"] = counts["p"]
+        for name, count in counts.items():
+            branches.truncate(name, len(branches.tokens[name]) - rng.choice((0, count - 1, rng.randint(0, count - 1))))
+        if turn % 3 == 2:
+            branches.step(**{name: 1 for name in branches.tokens})
+    for name in list(branches.tokens):
+        branches.release(name)
+    assert runner.cache.capacity().free_blocks == runner.cache.num_blocks
+    return branches
