@@ -475,6 +475,9 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
 
     own_tiles = -(-max_query * per_token // 16)
     own_parts = sequences * own_tiles * kv_heads
+    # (without a bound on what a sequence brings there would be a workgroup for every token of the
+    # batch in each: some turns of the chip share the tiles that there are)
+    sharing = min(own_tiles, max(1, 64 * units // (sequences * kv_heads)))
     if own_parts <= units and (max_shared + max_own) * 2 * head_dim * dtype.itemsize <= WHOLE_BYTES:
         return 16, 0, own_tiles, 0
     fewest_parts = -(-max_shared // 128)
@@ -498,7 +501,7 @@ def shared_prefix_launch(rows: int, groups: int, sequences: int, kv_heads: int, 
     def splits(wanted: float, keys: int) -> int:
         return max(1, min(round(wanted), -(-keys // (128 if few else 256)), _DECODE_MAX_SPLITS))
 
-    return tile, splits(room / parts, max_shared), own_tiles, splits((2 if few else 1) * units // own_parts, max_own)
+    return tile, splits(room / parts, max_shared), sharing, splits((2 if few else 1) * units // own_parts, max_own)
 
 
 def _bound(name: str, given: int | None, most: int) -> int:
