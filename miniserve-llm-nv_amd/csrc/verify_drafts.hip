@@ -21,8 +21,8 @@
 // are taken, by every workgroup of the request for itself, and the masses of a chunk of w and
 // p at the row where they end; (3) the draw: the chunk by the chunks' masses, then the token.
 //
-// (1) reads every logit once, and with some 22 64-bit instructions an element those and the
-// read take about as long: 576 rows of 151,936, 350 MB, 64 to 76 us = 4.6 to 5.5 TB/s on
+// (1) reads every logit once, and with 14 64-bit instructions an element those and the
+// read take about as long: 576 rows of 151,936, 350 MB, 65 to 76 us = 4.6 to 5.4 TB/s on
 // MI355X (a large copy: 4.9); with 64 requests of 8 drafts (2), (2a) and (3) take 33 us more.  One request of 4
 // drafts takes 6 + 6 + 6 us, each the chain of its loads and sums over a workgroup.  (With the
 // draw in (2), by the request's last workgroup, each has to make its masses visible to the
@@ -41,7 +41,7 @@ constexpr int kRowThreads = 256, kChooseThreads = 512, kDrawThreads = kChunk / 4
 // relative error there is least (found by exchange of its extrema: 4.0e-11 and 1.3e-14).  They
 // travel with a kernel's arguments, so that the coefficients lie in scalar registers: as literals
 // the compiler copies each into vector registers before every use (39 instructions an element
-// instead of 25).  The shorter one serves Z, the sum over all tokens of all rows (76 us for 576
+// instead of 25).  The shorter one serves Z, the sum over all tokens of all rows (73 us for 576
 // rows, with the longer one 89): it moves a border by 4e-11 of itself at most, past one uniform
 // number in some 10^10.
 constexpr int kDegree = 9, kSumDegree = 7;

@@ -47,8 +47,9 @@ class StepEntry:
 # one with drafted ones behind it): prompts go to the tiled kernel.  Measured on MI355X with 2
 # to 64 single tokens, head size 128, 8 kv heads, against each row reading its own keys: with
 # 1,024 shared keys and half or more spared the kernel takes 0.94 of the time at most and 0.5
-# at best (64 rows: 15.2 us against 30.5), with 256 keys 1 to 1.2 of it, and pairs, which
-# spare less than half, 0.9 to 1.3 up to 1,024 keys.
+# at best (64 rows: 15.2 us against 30.5), with 256 keys 1 to 1.2 of it.
+# Pairs spare less than half: several of them take 0.8 to 1.2 of the time at 1,024 to 16,384
+# keys, a lone pair 0.9 at 1,024, 0.8 to 0.96 at 4,096 and 0.75 at 16,384, which this rule leaves unused.
 SHARED_FRONT_KEYS = 512
 SHARED_FRONT_TOKENS = 16
 

@@ -443,7 +443,10 @@ def can_share_prefix(head_dim: int, block_size: int) -> bool:
 # compute unit at most, one kernel walks each sequence whole, without parts to join: a unit draws
 # some 40 KB a microsecond.  Measured on MI355X, 2 to 30 sequences, one kernel against parts and
 # their join: 65 KB 6.5 us against 9.2 recorded, 10.8 against 15.5 an eager call (the host's time);
-# 260 KB 11.2 against 9.6 and 10.8 against 15.5; 510 KB 17 against 10 and 15.7 against 15.5.
+# 260 KB 11.2 against 9.6 and 10.8 against 15.5; 510 KB 17 against 10 and 15.7 against 15.5.  The
+# bound goes by eager calls: recorded ones gain 2.7 us at 65 KB and lose 1.6 us at 260.  (A decode
+# step that shares keys has 512 of them or more and is cut by its recording's bounds, so it hardly
+# comes here.)
 WHOLE_BYTES = 300_000
 
 
@@ -548,7 +551,8 @@ def attention_shared_prefix(
     rounding.  A token that sees no key gives zeros, as do rows of
     ``q`` before the first sequence and behind the last.  Lengths beyond what a table's row
     names pages for count as that.  The caller guarantees that every page that the tables
-    name for the keys that are read lies inside the pool.
+    name for the keys that are read lies inside the pool, and that ``query_start`` and
+    ``group_start`` ascend from 0 or more to at most N and S.
 
     Takes float32 and bfloat16, head sizes in steps of 16 up to 128 and pages of a multiple
     of 16 keys (:func:`can_share_prefix`), and no window: a window hides most of a long
